@@ -1,0 +1,72 @@
+// Rows of 8-bit integers with a 32-bit scale each: row r stands for q[r, k] * scale[r].
+//
+//   A = max(max_k |x_k|, 127 * 2^-126),   scale = A / 127,   q_k = 127 x_k / A rounded to nearest even
+//
+// The quotient is rounded as if it were exact, so a row's integers are a function of its values alone,
+// whichever kernel made them.  (16-bit data has many quotients that end in one half: x = max / 2 gives 63.5.)
+// The floor under A keeps scale a normal number and 127 / A finite; a row of zeros gets zeros.
+// A row that holds a NaN or an infinity has no scale: it gets NaN, and zeros for q, so that whatever is
+// computed from the row is NaN instead of wrong.
+#pragma once
+#include "common.cuh"
+
+namespace skyla {
+namespace q8 {
+
+constexpr float kMost = 127.f;
+constexpr float kLeastMax = 127.f * 1.17549435e-38f;  // 127 * 2^-126: exact
+constexpr unsigned kInfBits = 0x7f800000u;
+constexpr float kNan = __builtin_nanf("");
+
+// |v| as bits: ordered like the values, an infinity above every number and a NaN above that
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct Step {
+  float most;  // A
+  float inv;   // 127 / A, rounded
+};
+__device__ __forceinline__ Step step_of(unsigned max_bits) {
+  Step s;
+  s.most = fmaxf(__uint_as_float(max_bits), kLeastMax);
+  s.inv = kMost / s.most;
+  return s;
+}
+
+// 127 x / A is nearer to one half than 32 bits can tell: 254 |x| against (2 k + 1) A decides, both exact in
+// 64 bits (k = the whole part).
+__device__ __noinline__ int round_close(float x, float most, float z) {
+  const int k = (int)fabsf(z);
+  const double two_x = 254.0 * (double)fabsf(x), edge = (double)(2 * k + 1) * (double)most;
+  const int n = two_x > edge ? k + 1 : (two_x < edge ? k : k + (k & 1));
+  return x < 0.f ? -n : n;
+}
+// z = x * inv is within 127 * 2^-23 < 2^-15 of the exact quotient (two roundings), so its nearest integer is
+// the exact quotient's unless z lies within 2^-15 of a half.
+__device__ __forceinline__ int round_q(float x, const Step& s) {
+  const float z = x * s.inv;
+  const float n = rintf(z);
+  if (fabsf(z - n) > 0.5f - 0x1p-15f) return round_close(x, s.most, z);
+  return (int)n;
+}
+
+// A product's sum with its two scales, in one order and never contracted into an addition that follows: every
+// kernel of the 8-bit product gives the same bits.
+__device__ __forceinline__ float scaled(int acc, float x_scale, float w_scale) {
+  return __fmul_rn(__fmul_rn(__int2float_rn(acc), x_scale), w_scale);
+}
+
+// Largest of a block's values, given to every thread; `scratch` holds 32 words.
+__device__ __forceinline__ unsigned block_max(unsigned v, unsigned* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n_warps = (blockDim.x + 31) >> 5;
+  v = __reduce_max_sync(0xffffffffu, v);
+  __syncthreads();
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  unsigned m = 0;
+  for (int i = 0; i < n_warps; ++i) m = max(m, scratch[i]);
+  return m;
+}
+
+}  // namespace q8
+}  // namespace skyla

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -583,6 +583,204 @@ def gemm_prompt(x: torch.Tensor, w_map: TensorMap, n_out: int, y: torch.Tensor, 
     share, flags, n_share = st.prompt_shares() if cut_k else (None, None, 0)
     _check("gemm_prompt", f(xm.buf, w_map.buf, ym, _ptr(y), _rows(y, "y"), m, n_out, k, mode, _ptr(st.error_flag),
                             *scale_args, *ahead_args, *prep_args, _ptr(share), _ptr(flags), n_share, _stream()))
+    return y
+
+
+# ------------------------------------------------------------- rows in 8 bits
+#: the widest rows whose products are exact in 32 bits: 131,071 products of at most 2^14
+Q8_MAX_WIDTH = 131071
+
+
+class Q8Rows(NamedTuple):
+    """Rows of 8-bit integers with a scale each: row r stands for ``q[r] * scale[r]``.
+
+    ``q``: int8 [rows, width], the elements of a row side by side (:func:`q8_rows` makes rows that begin on
+    multiples of 16 bytes, which the tensor-core product wants); ``scale``: float32 [rows].  A row made from
+    values with a NaN or an infinity among them has the scale NaN."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+def q8_rows(n: int, width: int, device) -> Q8Rows:
+    """Room for ``n`` rows of ``width`` (not initialised)."""
+    q = torch.empty((n, -(-width // 16) * 16), dtype=torch.int8, device=device)
+    return Q8Rows(q if q.shape[1] == width else q[:, :width], torch.empty(n, dtype=torch.float32, device=device))
+
+
+def _q8(rows: Q8Rows, what: str) -> int:
+    """Row stride of 8-bit rows, after their check."""
+    q, scale = rows
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise KernelError(f"{what}: 8-bit rows are int8 with float32 scales, not {q.dtype} and {scale.dtype}")
+    ld = _rows(q, what)
+    if scale.dim() != 1 or scale.shape[0] != q.shape[0] or not scale.is_contiguous():
+        raise KernelError(f"{what}: one contiguous scale per row, got {tuple(scale.shape)} for rows {tuple(q.shape)}")
+    return ld
+
+
+def _written(ld: int, t: torch.Tensor, what: str) -> int:
+    """The row stride of a matrix that a kernel writes: its rows must not lie on one another."""
+    if ld < t.shape[1] and t.shape[0] > 1:
+        raise KernelError(f"{what}: rows of {t.shape[1]} elements {ld} apart would be written over one another")
+    return ld
+
+
+def _device_of(*tensors) -> int:
+    """The one CUDA device of the operands."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if not t.is_cuda:
+            raise KernelError("kernel operands must be CUDA tensors; there is no host path")
+        if t.get_device() != dev:
+            raise KernelError(f"kernel operands on devices {dev} and {t.get_device()}")
+    return dev
+
+
+def _launch_on(dev: int, module: str, f, *args) -> None:
+    """Launch on the operands' device, whichever is current, on its current stream."""
+    if dev == torch.cuda.current_device():
+        _check(module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            _check(module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+
+
+def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
+    """Each row of ``x`` (bfloat16 or float32, [rows, width]) in 8 bits: ``scale = max|x| / 127`` and
+    ``q = x / scale``, the exact quotient rounded to the nearest integer (ties to even).
+
+    A row of zeros stays zeros; a row that holds a NaN or an infinity gets the scale NaN and zeros."""
+    ld, code = _rows(x, "quantize_rows"), dtype_code(x)
+    n, width = x.shape
+    if out is None:
+        out = q8_rows(n, width, x.device)
+    if out.q.shape != x.shape:
+        raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(out.q.shape)}")
+    ldq = _written(_q8(out, "quantize_rows"), out.q, "quantize_rows")
+    dev = _device_of(x, out.q, out.scale)
+    f = _fn("quant", "skyla_quantize_rows",
+            [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p])
+    _launch_on(dev, "quant", f, x.data_ptr(), code, ld, n, width, out.q.data_ptr(), ldq, out.scale.data_ptr())
+    return out
+
+
+def dequantize_rows(rows: Q8Rows, out: torch.Tensor) -> torch.Tensor:
+    """What 8-bit rows stand for: ``out[r] = q[r] * scale[r]`` in ``out``'s type (bfloat16 or float32)."""
+    ldq, ldo, code = _q8(rows, "dequantize_rows"), _rows(out, "dequantize_rows"), dtype_code(out)
+    if rows.q.shape != out.shape:
+        raise KernelError(f"dequantize_rows: rows {tuple(rows.q.shape)} do not go into {tuple(out.shape)}")
+    _written(ldo, out, "dequantize_rows")
+    dev = _device_of(rows.q, rows.scale, out)
+    f = _fn("quant", "skyla_dequantize_rows",
+            [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p])
+    _launch_on(dev, "quant", f, rows.q.data_ptr(), ldq, rows.scale.data_ptr(), out.shape[0], out.shape[1],
+               out.data_ptr(), code, ldo)
+    return out
+
+
+def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[Q8Rows] = None,
+               residual: Optional[torch.Tensor] = None) -> Q8Rows:
+    """``rmsnorm(x) * weight`` in 8-bit rows, computed in 32 bits; with ``residual`` the rows are added into ``x``
+    first (``x`` is written, in its own type, and the norm is that of the sum as it is kept).
+
+    ``x`` and ``residual``: bfloat16 or float32.  A row whose sum of squares or whose products with the weight
+    leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row of zeros with ``eps = 0``."""
+    ld, code = _rows(x, "rmsnorm_q8"), dtype_code(x)
+    n, width = x.shape
+    if weight.dtype != torch.float32 or weight.dim() != 1 or not weight.is_contiguous() or weight.shape[0] != width:
+        raise KernelError(f"rmsnorm_q8: the weight must be a contiguous float32 vector of {width}")
+    if not eps >= 0:
+        raise KernelError(f"rmsnorm_q8: eps must not be negative, got {eps}")
+    if out is None:
+        out = q8_rows(n, width, x.device)
+    if out.q.shape != x.shape:
+        raise KernelError(f"rmsnorm_q8: rows {tuple(x.shape)} do not go into {tuple(out.q.shape)}")
+    ldq = _written(_q8(out, "rmsnorm_q8"), out.q, "rmsnorm_q8")
+    ldr = rcode = r_ptr = 0
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise KernelError(f"rmsnorm_q8: residual {tuple(residual.shape)} against x {tuple(x.shape)}")
+        ldr, rcode, r_ptr = _rows(residual, "rmsnorm_q8"), dtype_code(residual), residual.data_ptr()
+        _written(ld, x, "rmsnorm_q8")
+        dev = _device_of(x, weight, out.q, out.scale, residual)
+    else:
+        dev = _device_of(x, weight, out.q, out.scale)
+    f = _fn("quant", "skyla_rmsnorm_q8",
+            [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_float, c_void_p, c_int64,
+             c_void_p, c_void_p])
+    _launch_on(dev, "quant", f, x.data_ptr(), code, ld, r_ptr, rcode, ldr, n, width, weight.data_ptr(), eps,
+               out.q.data_ptr(), ldq, out.scale.data_ptr())
+    return out
+
+
+class Q8Weight:
+    """A weight [outputs, inputs] in 8 bits with a scale per output, as :func:`linear_q8` reads it.
+
+    ``gated``: all gate rows, then the up rows of the same outputs.  The tensors are kept as they are if the rows
+    begin on multiples of 16 bytes, else copied into such rows.  The product's kernels ask for the weight before
+    they wait for the kernels ahead of them, so it is finished for good: the constructor waits for the current
+    stream, and nobody writes the tensors afterwards."""
+
+    __slots__ = ("rows", "gated", "n_out", "n_in", "ld")
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, gated: bool = False):
+        ld = _q8(Q8Rows(q, scale), "Q8Weight")
+        n, width = q.shape
+        if not 1 <= width <= Q8_MAX_WIDTH:
+            raise KernelError(f"Q8Weight: {width} inputs are outside 1..{Q8_MAX_WIDTH}")
+        if n < 1 or (gated and n % 2):
+            raise KernelError(f"Q8Weight: {n} rows" + (" do not divide into gate and up" if gated else ""))
+        if ld % 16 or ld < width or q.data_ptr() % 16:
+            kept = q8_rows(n, width, q.device).q
+            kept.copy_(q)
+            q, ld = kept, _rows(kept, "Q8Weight")
+        if q.is_cuda:
+            torch.cuda.current_stream(q.device).synchronize()
+        self.rows, self.gated, self.n_in, self.ld = Q8Rows(q, scale), bool(gated), width, ld
+        self.n_out = n // 2 if gated else n
+
+    @classmethod
+    def quantize(cls, weight: torch.Tensor, gated: bool = False) -> "Q8Weight":
+        """A bfloat16 or float32 weight in 8 bits, each row (output) with its own scale."""
+        return cls(*quantize_rows(weight), gated=gated)
+
+    def first_outputs(self, n: int) -> "Q8Weight":
+        """The weight of the first ``n`` outputs, sharing this one's memory."""
+        if self.gated or not 1 <= n <= self.n_out:
+            raise KernelError(f"Q8Weight: the first {n} of {self.n_out} outputs" + (" of a gated weight" if self.gated else ""))
+        return Q8Weight(self.rows.q[:n], self.rows.scale[:n])
+
+    def bytes(self) -> int:
+        return self.rows.q.shape[0] * (self.n_in + 4)
+
+
+def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
+              state: Optional[KernelState] = None) -> torch.Tensor:
+    """The product of tokens and a weight in 8 bits: ``v[t, n] = (sum_k x.q[t, k] w.q[n, k]) x.scale[t] w.scale[n]``,
+    the sum exact, the scales applied in 32 bits.
+
+    ``mode``: STORE (``y = v``, bfloat16 or float32), ACCUMULATE (``y += v``, float32), GATED (``y = silu(gate) * up``
+    of a gated weight, bfloat16).  ``x``'s rows should begin on multiples of 16 bytes (as :func:`q8_rows` makes
+    them): others run on the plain kernel, with the same results."""
+    ldx = _q8(x, "linear_q8")
+    m, k = x.q.shape
+    if k != w.n_in:
+        raise KernelError(f"linear_q8: tokens of {k} against a weight of {w.n_in} inputs")
+    if mode not in (STORE, ACCUMULATE, GATED) or (mode == GATED) != w.gated:
+        raise KernelError(f"linear_q8: mode {mode} on a weight that is {'' if w.gated else 'not '}gated")
+    ldy, code = _rows(y, "linear_q8"), dtype_code(y)
+    if tuple(y.shape) != (m, w.n_out):
+        raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
+    if (mode == ACCUMULATE and code != F32) or (mode == GATED and code != BF16):
+        raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
+    _written(ldy, y, "linear_q8")
+    dev = _device_of(x.q, x.scale, w.rows.q, w.rows.scale, y)
+    f = _fn("linear_q8_plain", "skyla_linear_q8_plain",
+            [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int64, c_int,
+             c_void_p])
+    _launch_on(dev, "linear_q8_plain", f, x.q.data_ptr(), ldx, x.scale.data_ptr(), w.rows.q.data_ptr(), w.ld,
+               w.rows.scale.data_ptr(), m, w.n_out, k, y.data_ptr(), code, ldy, mode)
     return y
 
 

@@ -1,0 +1,76 @@
+"""What the 8-bit operators refuse, and how a weight in 8 bits is laid out, without a GPU."""
+import pytest
+import torch
+
+from skyla_kernel_b200.kernels import ops
+
+
+def _rows(n, k, pad=0):
+    q = torch.zeros(n, k + pad, dtype=torch.int8)[:, :k]
+    return ops.Q8Rows(q, torch.ones(n))
+
+
+def test_rows_begin_on_multiples_of_16_bytes():
+    for n, k in ((1, 1), (3, 16), (5, 17), (2, 100)):
+        r = ops.q8_rows(n, k, "cpu")
+        assert r.q.shape == (n, k) and r.q.stride(0) % 16 == 0 and r.q.dtype == torch.int8
+        assert r.scale.shape == (n,) and r.scale.dtype == torch.float32
+
+
+def test_a_weight_is_kept_or_laid_out():
+    aligned = ops.q8_rows(6, 33, "cpu")
+    aligned.q.copy_(torch.arange(6 * 33).reshape(6, 33) % 100)
+    w = ops.Q8Weight(*aligned)
+    assert w.rows.q.data_ptr() == aligned.q.data_ptr() and (w.n_out, w.n_in, w.ld) == (6, 33, 48)
+    packed = aligned.q.contiguous()                      # rows of 33 bytes: copied
+    v = ops.Q8Weight(packed, aligned.scale, gated=True)
+    assert v.rows.q.data_ptr() != packed.data_ptr() and torch.equal(v.rows.q, packed) and v.ld % 16 == 0
+    assert (v.n_out, v.gated, v.bytes()) == (3, True, 6 * 37)
+    part = w.first_outputs(2)
+    assert part.rows.q.data_ptr() == w.rows.q.data_ptr() and part.n_out == 2
+    broadcast = ops.Q8Weight(packed[:1].expand(4, 33), torch.ones(4))  # one row for all outputs: copied as well
+    assert broadcast.ld % 16 == 0 and torch.equal(broadcast.rows.q, packed[:1].expand(4, 33))
+
+
+@pytest.mark.parametrize("make", [
+    lambda: ops.Q8Weight(torch.zeros(4, 8, dtype=torch.uint8), torch.ones(4)),
+    lambda: ops.Q8Weight(torch.zeros(4, 8, dtype=torch.int8), torch.ones(3)),
+    lambda: ops.Q8Weight(torch.zeros(4, 8, dtype=torch.int8), torch.ones(4, dtype=torch.bfloat16)),
+    lambda: ops.Q8Weight(torch.zeros(3, 8, dtype=torch.int8), torch.ones(3), gated=True),
+    lambda: ops.Q8Weight(torch.zeros(0, 8, dtype=torch.int8), torch.ones(0)),
+    lambda: ops.Q8Weight(torch.zeros(1, ops.Q8_MAX_WIDTH + 1, dtype=torch.int8), torch.ones(1)),
+    lambda: ops.Q8Weight(torch.zeros(8, 4, dtype=torch.int8).T, torch.ones(4)),
+    lambda: ops.Q8Weight(*_rows(4, 16), gated=True).first_outputs(1),
+    lambda: ops.Q8Weight(*_rows(4, 16)).first_outputs(5),
+    # quantisation
+    lambda: ops.quantize_rows(torch.zeros(2, 3, 4)),
+    lambda: ops.quantize_rows(torch.zeros(2, 3, dtype=torch.float16)),
+    lambda: ops.quantize_rows(torch.zeros(2, 3), _rows(2, 4)),
+    lambda: ops.quantize_rows(torch.zeros(2, 3), ops.Q8Rows(torch.zeros(1, 3, dtype=torch.int8).expand(2, 3), torch.ones(2))),
+    lambda: ops.dequantize_rows(_rows(2, 3), torch.zeros(2, 4)),
+    lambda: ops.dequantize_rows(_rows(2, 3), torch.zeros(1, 3).expand(2, 3)),
+    lambda: ops.dequantize_rows(ops.Q8Rows(torch.zeros(2, 3, dtype=torch.int8), torch.ones(4)[::2]), torch.zeros(2, 3)),
+    # norm
+    lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(7), 1e-6),
+    lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8, dtype=torch.bfloat16), 1e-6),
+    lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), 1e-6, residual=torch.zeros(1, 8)),
+    lambda: ops.rmsnorm_q8(torch.zeros(1, 8).expand(2, 8), torch.ones(8), 1e-6, residual=torch.zeros(2, 8)),
+    lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), -1e-6),
+    lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), float("nan")),
+    # product
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 32)), torch.zeros(2, 4)),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 5)),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 4), ops.GATED),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16), gated=True), torch.zeros(2, 2, dtype=torch.bfloat16)),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16), gated=True), torch.zeros(2, 2), ops.GATED),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 4, dtype=torch.bfloat16), ops.ACCUMULATE),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 4), 7),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(1, 4).expand(2, 4)),
+    # all of them on the host
+    lambda: ops.quantize_rows(torch.zeros(2, 3)),
+    lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), 1e-6),
+    lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 4)),
+])
+def test_refusals(make):
+    with pytest.raises(ops.KernelError):
+        make()
