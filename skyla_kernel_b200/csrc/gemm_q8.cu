@@ -1,0 +1,923 @@
+// The matrix product of two sets of 8-bit rows (q8.cuh) on the tensor cores: tokens x [M, K] and a weight
+// W [N, K] (rows are outputs), both K-major, each row with a scale of its own.
+//   acc[t, f] = sum_k x[t, k] W[f, k]   tcgen05.mma kind::i8, 32-bit integers in TMEM: exact in every order, so
+//                                       how a product is cut never shows in its result
+//   v = acc * x_scale[t] * w_scale[f]   y = v, y += v, or y = silu(v of the gate) * v of the up
+// Two kernels, as for bfloat16 (gemm_tc.cu, gemm_prompt.cu); a K block is 128 bytes, one swizzle row, here 128
+// elements, and an instruction takes 32 of them:
+//   up to 128 tokens  the weight streams through every SM once; the weight's rows are the MMA's 128 rows and the
+//                     tokens its columns;
+//   more              the tokens are the MMA's rows, so that a thread of the epilogue owns a token's row.
+// Every mbarrier wait is bounded: on a timeout the block records an error code (1 to 19), lets the loads it issued
+// land, frees its TMEM and returns.
+#include <cuda.h>
+
+#include <cstring>
+
+#include "q8.cuh"
+#include "tc_common.cuh"
+using namespace skyla;
+SKYLA_EXPORT_ERROR_MESSAGE()
+
+namespace {
+using namespace skyla::tc;
+using skyla::q8::scaled;
+
+enum Mode : int { kStoreBf16 = 0, kStoreF32 = 1, kAccumF32 = 2, kGluBf16 = 3 };
+
+constexpr int BM = 128;      // rows of an MMA
+constexpr int KB = 128;      // bytes, and elements, of a K block
+constexpr int kThreads = 192;
+constexpr int kMaxWidth = 131071;  // products of at most 2^14 whose sums stay within 32 bits
+
+struct Args {
+  void* y; int64_t ldy;
+  int M, N, K;
+  const float* x_scale; const float* w_scale;  // [M], [N] (2N gated)
+  int* error_flag;
+};
+
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D 32-bit integers, A and B signed 8-bit, both K-major, N columns, M = 128
+__device__ __forceinline__ uint32_t idesc_i8(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&p);
+}
+// With the fast exponential and division: their error (a few 2^-22, 2^-17 far from zero) is well below the
+// bfloat16 rounding that follows.
+__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+// ---------------------------------------------------------------------------------- few tokens: weight streaming
+// The structure of the bfloat16 kernel of the same kind (gemm_tc.cu, where its measurements stand): one box brings
+// `kkb` K blocks of a tile of R weight rows; tiles are cut so that every SM streams; short tiles stack `kstack` K
+// blocks into one MMA, whose diagonal blocks are the partial sums; from 17 tokens on K is cut into a thread-block
+// cluster whose blocks exchange their tiles by bulk copies through distributed shared memory.
+constexpr int kRowsMaxStages = 24;
+constexpr int kRowsSmemBytes = 212 * 1024;
+
+struct RowsArgs {
+  int rows_per_block, n_stages, kkb, kstack, tmem_cols;
+  int kb_per_split;
+};
+
+enum RowsKind : int { kPlain = 0, kCluster = 1, kStacked = 2 };
+template <int BN, int MODE, int KIND>
+__global__ void __launch_bounds__(kThreads, 1)
+q8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args a,
+               const RowsArgs ra) {
+  constexpr int kATiles = MODE == kGluBf16 ? 2 : 1;
+  constexpr int kBBytes = BN * KB;
+  constexpr bool clustered = KIND == kCluster;
+  constexpr bool stacked = KIND == kStacked;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ float tok_scale[BN];
+
+  const int n_stages = ra.n_stages, kkb = ra.kkb, R = ra.rows_per_block;
+  const int a_tile = R * KB;  // R rows of 128 bytes: a multiple of 1024
+  const uint32_t stage_bytes = (uint32_t)(kkb * (kATiles * a_tile + kBBytes));
+  const uint32_t bars = (smem_u32(smem_raw) + 15u) & ~15u;
+  const uint32_t base = (bars + 8u * (2 * kRowsMaxStages + 3) + 1023u) & ~1023u;
+  const uint32_t landing = base + (uint32_t)n_stages * stage_bytes;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kRowsMaxStages + s); };
+  const uint32_t tmem_full_bar = bars + 8u * (2 * kRowsMaxStages);
+  const uint32_t land_bar = bars + 8u * (2 * kRowsMaxStages + 1);
+  const uint32_t sent_bar = bars + 8u * (2 * kRowsMaxStages + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int f0 = blockIdx.x * R;
+  const int total_kb = (a.K + KB - 1) / KB;
+  const int kb0 = blockIdx.z * ra.kb_per_split;
+  const int n_kb = max(0, min(ra.kb_per_split, total_kb - kb0));
+  const int n_st = (n_kb + kkb - 1) / kkb;
+  // every block walks its stages from a start of its own, so that the blocks read different lines of the tokens' rows
+  const int st_start = n_st > 0 ? (int)(((unsigned)blockIdx.x * 5u) % (unsigned)n_st) : 0;
+  auto st_of = [&](int i) { int t = i + st_start; return t >= n_st ? t - n_st : t; };
+  const uint32_t tx_bytes = (uint32_t)(kkb * kATiles * a_tile) + (uint32_t)(kkb * kBBytes);
+
+  auto load_weights = [&](int i, int s) {
+    const uint32_t sa = base + s * stage_bytes;
+    const int kb = kb0 + st_of(i) * kkb;
+    mbar_expect_tx(full_bar(s), tx_bytes);
+    if (kkb == 1) {
+      tma_load_2d(sa, &map_w, full_bar(s), kb * KB, f0);
+      if (MODE == kGluBf16) tma_load_2d(sa + a_tile, &map_w, full_bar(s), kb * KB, a.N + f0);
+    } else {
+      tma_load_3d(sa, &map_w, full_bar(s), 0, f0, kb);
+      if (MODE == kGluBf16) tma_load_3d(sa + kkb * a_tile, &map_w, full_bar(s), 0, a.N + f0, kb);
+    }
+  };
+  uint32_t my_rank = 0, n_ranks = 1;
+  if (clustered) {
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(my_rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_ranks));
+  }
+  // K splits as a cluster: rank r owns the tokens [r * per, r * per + per) of the tile
+  const int per = (a.M + (int)n_ranks - 1) / (int)n_ranks;
+  const int owners = (a.M + per - 1) / per;
+  const int n_dst = owners - ((int)my_rank < owners ? 1 : 0);  // peers that this block sends tokens to
+  const int n_pre = min(n_st, n_stages);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < n_stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(tmem_full_bar, 1);
+    mbar_init(land_bar, 1);
+    mbar_init(sent_bar, n_dst > 0 ? n_dst : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // weights are finished before any launch that reads them (the caller's weight object waits for them), so the
+    // ring's first filling is asked for at once
+    for (int i = 0; i < n_pre; ++i) load_weights(i, i);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_slot)), "r"((uint32_t)ra.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_base_slot;
+  allow_dependents();
+  // nobody may send into a peer's landing zone before that peer's barrier exists: all arrive here, senders wait later
+  if (clustered) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  bool met_cluster = false;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      auto load_tokens = [&](int i, int s) {
+        const uint32_t sb = base + s * stage_bytes + kkb * kATiles * a_tile;
+        const int kb = kb0 + st_of(i) * kkb;
+        if (kkb == 1) tma_load_2d(sb, &map_x, full_bar(s), kb * KB, 0);
+        else tma_load_3d(sb, &map_x, full_bar(s), 0, 0, kb);
+      };
+      grid_dependency_wait();
+      for (int i = 0; i < n_pre; ++i) load_tokens(i, i);
+      int i = n_pre, s = 0;
+      uint32_t phase = 1;
+      for (; i < n_st; ++i) {
+        if (!mbar_wait(empty_bar(s), phase ^ 1, &abort_flag, a.error_flag, 1)) break;
+        load_weights(i, s);
+        load_tokens(i, s);
+        if (++s == n_stages) { s = 0; phase ^= 1; }
+      }
+      if (i < n_st) {  // gave up: let the loads in flight land before the block's memory goes away
+        for (int j = max(0, i - n_stages); j < i; ++j) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(full_bar(j % n_stages), (j / n_stages) & 1) && clock64() - t0 < kWaitCycles) {}
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const int kstack = stacked ? ra.kstack : 1;
+      const uint32_t idesc = idesc_i8(kstack * BN);
+      int s = 0;
+      uint32_t phase = 0, started = 0;
+      for (int i = 0; i < n_st; ++i) {
+        if (!mbar_wait(full_bar(s), phase, &abort_flag, a.error_flag, 2)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sa = base + s * stage_bytes, sb = sa + kkb * kATiles * a_tile;
+        // K blocks past the end of K hold zeros (the loads fill them)
+        for (int j = 0; j < kkb; j += kstack) {
+          const uint64_t da = umma_desc(sa + j * a_tile), db = umma_desc(sb + j * kBBytes);
+          const uint64_t du = umma_desc(sa + (kkb + j) * a_tile);
+#pragma unroll
+          for (int k = 0; k < KB / 32; ++k) {
+            umma_i8(tmem_base, da + 2 * k, db + 2 * k, idesc, started);
+            if (MODE == kGluBf16) umma_i8(tmem_base + BN, du + 2 * k, db + 2 * k, idesc, started);
+            started = 1u;
+          }
+        }
+        umma_commit(empty_bar(s));
+        if (++s == n_stages) { s = 0; phase ^= 1; }
+      }
+      umma_commit(tmem_full_bar);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue warps
+    const int quad = warp & 3;
+    const int r_local = quad * 32 + lane;  // row of the tile that this thread's TMEM lane holds
+    const int f = f0 + r_local;
+    const bool mine = r_local < R && f < a.N;
+    const int et = threadIdx.x - 64;
+    // what does not depend on the product is fetched while the main loop runs
+    const float ws = mine ? a.w_scale[f] : 0.f;
+    const float us = MODE == kGluBf16 && mine ? a.w_scale[a.N + f] : 0.f;
+    grid_dependency_wait();
+    if (et < BN) tok_scale[et] = et < a.M ? a.x_scale[et] : 0.f;
+    const int kstack = stacked ? ra.kstack : 1;
+    int* red = reinterpret_cast<int*>(smem_raw + (landing - smem_u32(smem_raw)));
+    float old_pre[4] = {0.f, 0.f, 0.f, 0.f}, old16[16];
+    if (MODE == kAccumF32 && stacked) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int idx = et + 128 * n;
+        const int tok = idx / R, ff = f0 + idx - tok * R;
+        if (idx < a.M * R && ff < a.N) old_pre[n] = ((const float*)a.y)[(int64_t)tok * a.ldy + ff];
+      }
+    }
+    if (MODE == kAccumF32 && KIND == kPlain && mine) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) old16[j] = j < a.M ? ((const float*)a.y)[(int64_t)j * a.ldy + f] : 0.f;
+    }
+    const int my_n = max(0, min(per, a.M - (int)my_rank * per));
+    constexpr uint32_t kRowBytes = BM * 4;  // a token's 128 outputs of the tile
+    // in a cluster's owner a warp takes every fourth token and a lane four neighbouring outputs of the tile
+    const int f4 = f0 + 4 * lane;
+    const bool mine4 = 4 * lane < R && f4 < a.N;  // (R and N are multiples of 4 there)
+    float4 old4[4], ws4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (clustered) {
+      if (et == 0 && my_n > 0) mbar_expect_tx(land_bar, (n_ranks - 1) * (uint32_t)my_n * kRowBytes);
+      if (mine4) ws4 = make_float4(a.w_scale[f4], a.w_scale[f4 + 1], a.w_scale[f4 + 2], a.w_scale[f4 + 3]);
+      if (MODE == kAccumF32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = quad + 4 * j;
+          old4[j] = (mine4 && i < my_n) ? *reinterpret_cast<const float4*>((const float*)a.y + (int64_t)((int)my_rank * per + i) * a.ldy + f4)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+    }
+    asm volatile("barrier.sync 1, 128;" ::: "memory");  // the tokens' scales
+    const bool ok = n_kb > 0 && mbar_wait(tmem_full_bar, 0, &abort_flag, a.error_flag, 3);
+    if (ok) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16);
+    if (clustered) {
+      // Every split writes its accumulator, token by token, into shared memory of its own (the ring, idle by now),
+      // one region per owner, and sends each region to its owner's landing zone with one bulk copy, which the
+      // owner's barrier counts in.  Columns past the last token are written too: nobody reads them.
+      const bool warp_reads = ok && quad * 32 < R;  // uniform for the warp
+      const uint32_t travel = base + 4u * (uint32_t)r_local;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN && warp_reads; c0 += 16) {
+        if (c0 >= a.M) break;
+        uint32_t r[16];
+        tmem_ld16(taddr + c0, r);
+        tmem_wait_ld();
+        const uint32_t at = travel + (uint32_t)c0 * kRowBytes;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + (uint32_t)j * kRowBytes), "r"(r[j]) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every peer's barrier exists from here on
+      met_cluster = true;
+      if (et == 0) {
+        for (uint32_t d = 1; ok && d < n_ranks; ++d) {
+          const uint32_t dst = (my_rank + d) % n_ranks;
+          const int dst_n = max(0, min(per, a.M - (int)dst * per));
+          if (dst_n == 0) continue;
+          uint32_t remote_zone, remote_bar;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote_zone) : "r"(landing + my_rank * (uint32_t)per * kRowBytes), "r"(dst));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote_bar) : "r"(land_bar), "r"(dst));
+          asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(remote_zone), "r"(base + dst * (uint32_t)per * kRowBytes), "r"((uint32_t)dst_n * kRowBytes), "r"(remote_bar)
+                       : "memory");
+        }
+      }
+      bool landed = ok;
+      if (landed && my_n > 0) landed = mbar_wait(land_bar, 0, &abort_flag, a.error_flag, 7);
+      if (et == 32 && landed && my_n > 0) {  // what the peers sent has arrived: they may leave
+        for (uint32_t d = 1; d < n_ranks; ++d) {
+          uint32_t remote_bar;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote_bar) : "r"(sent_bar), "r"((my_rank + d) % n_ranks));
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
+        }
+      }
+      const uint32_t rank_stride = (uint32_t)per * kRowBytes;
+      const uint32_t zone = landing + 16u * (uint32_t)lane;                      // [source rank][owned token][output]
+      const uint32_t own = base + my_rank * rank_stride + 16u * (uint32_t)lane;  // this block's own share of its tokens
+#pragma unroll 1
+      for (int j = 0; quad + 4 * j < my_n; ++j) {
+        const int i = quad + 4 * j, col = (int)my_rank * per + i;
+        if (!landed || !mine4) continue;
+        int4 sum = make_int4(0, 0, 0, 0);
+        for (uint32_t src = 0; src < n_ranks; ++src) {
+          int4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"((src == my_rank ? own : zone + src * rank_stride) + (uint32_t)i * kRowBytes));
+          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        const float xs = tok_scale[col];
+        const float4 v = make_float4(scaled(sum.x, xs, ws4.x), scaled(sum.y, xs, ws4.y), scaled(sum.z, xs, ws4.z), scaled(sum.w, xs, ws4.w));
+        if (MODE == kStoreBf16) {
+          *reinterpret_cast<uint2*>((__nv_bfloat16*)a.y + (int64_t)col * a.ldy + f4) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+        } else if (MODE == kStoreF32) {
+          *reinterpret_cast<float4*>((float*)a.y + (int64_t)col * a.ldy + f4) = v;
+        } else {
+          float* p = (float*)a.y + (int64_t)col * a.ldy + f4;
+          const float4 o = j == 0 ? old4[0] : j == 1 ? old4[1] : j == 2 ? old4[2] : j == 3 ? old4[3] : *reinterpret_cast<const float4*>(p);
+          *reinterpret_cast<float4*>(p) = make_float4(__fadd_rn(o.x, v.x), __fadd_rn(o.y, v.y), __fadd_rn(o.z, v.z), __fadd_rn(o.w, v.w));
+        }
+      }
+    } else if (stacked) {
+      // lane L of the accumulator is row L % R of K-block group L / R; its partial sums are the columns
+      // [q * BN, q * BN + BN) of its own group q.  red[(q * BN + tok) * R + r], then a sum over q.
+      if (ok) {
+        const int L = quad * 32 + lane;
+        const int q_mine = L / R, r_mine = L - q_mine * R;
+        const int q_lo = (quad * 32) / R, q_hi = min(kstack - 1, (quad * 32 + 31) / R);  // uniform for the warp
+        for (int q = q_lo; q <= q_hi; ++q) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < BN; c0 += 16) {
+            if (c0 >= a.M) break;
+            uint32_t r[16];
+            tmem_ld16(taddr + q * BN + c0, r);
+            tmem_wait_ld();
+            if (q == q_mine) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (c0 + j < a.M) red[(q * BN + c0 + j) * R + r_mine] = (int)r[j];
+            }
+          }
+        }
+      }
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
+      const float inv_R = 1.0f / (float)R;
+      for (int idx = et; ok && idx < a.M * R; idx += 128) {
+        // idx / R without the integer division: (idx + 0.5) / R is at least 1 / (2 R) away from an integer
+        const int tok = (int)(((float)idx + 0.5f) * inv_R), rr = idx - tok * R;
+        const int ff = f0 + rr;
+        if (ff >= a.N) continue;
+        int sum = 0;
+        for (int q = 0; q < kstack; ++q) sum += red[(q * BN + tok) * R + rr];
+        const float v = scaled(sum, tok_scale[tok], a.w_scale[ff]);
+        if (MODE == kStoreBf16) ((__nv_bfloat16*)a.y)[(int64_t)tok * a.ldy + ff] = __float2bfloat16_rn(v);
+        else if (MODE == kStoreF32) ((float*)a.y)[(int64_t)tok * a.ldy + ff] = v;
+        else {
+          float* p = (float*)a.y + (int64_t)tok * a.ldy + ff;
+          const int n = (idx - et) >> 7;  // which of this thread's items
+          *p = __fadd_rn(n == 0 ? old_pre[0] : n == 1 ? old_pre[1] : n == 2 ? old_pre[2] : n == 3 ? old_pre[3] : *p, v);
+        }
+      }
+    } else {
+      const bool warp_has_rows = ok && quad * 32 < R;  // uniform for the warp
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN && warp_has_rows; c0 += 16) {
+        if (c0 >= a.M) break;
+        uint32_t r[16], u[16];
+        __syncwarp();
+        tmem_ld16(taddr + c0, r);
+        if (MODE == kGluBf16) tmem_ld16(taddr + BN + c0, u);
+        tmem_wait_ld();
+        if (!mine) continue;
+        float old[16];
+        if (MODE == kAccumF32) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            old[j] = c0 == 0 ? old16[j] : (c0 + j < a.M ? ((const float*)a.y)[(int64_t)(c0 + j) * a.ldy + f] : 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int tok = c0 + j;
+          if (tok >= a.M) break;
+          const float v = scaled((int)r[j], tok_scale[tok], ws);
+          if (MODE == kStoreBf16) ((__nv_bfloat16*)a.y)[(int64_t)tok * a.ldy + f] = __float2bfloat16_rn(v);
+          else if (MODE == kStoreF32) ((float*)a.y)[(int64_t)tok * a.ldy + f] = v;
+          else if (MODE == kAccumF32) ((float*)a.y)[(int64_t)tok * a.ldy + f] = __fadd_rn(old[j], v);
+          else ((__nv_bfloat16*)a.y)[(int64_t)tok * a.ldy + f] = __float2bfloat16_rn(silu_times(v, scaled((int)u[j], tok_scale[tok], us)));
+        }
+      }
+    }
+  }
+  if (clustered) {
+    // A block's shared memory has to outlive the copies that read it: it leaves when every peer that it sent to has
+    // told it so.  A peer that gave up never tells; the wait is bounded like every other.
+    if (!met_cluster) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (threadIdx.x == 64 && n_dst > 0 && !abort_flag) mbar_wait(sent_bar, 0, &abort_flag, a.error_flag, 8);
+  }
+  // ------------------------------------------------------------------ teardown
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0 && n_kb > 0) {  // the accumulator must be idle before its columns are freed
+      const long long t0 = clock64();
+      while (!mbar_try_wait(tmem_full_bar, 0) && clock64() - t0 < kWaitCycles) {}
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)ra.tmem_cols) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------- many tokens
+// One block per SM walks tiles of 128 tokens x BF accumulator columns (a gated weight: BF / 2 gate rows and the BF / 2
+// up rows of the same outputs), two accumulators in turn: the epilogue of one tile runs beside the products of the
+// next.  warp 0 loads, warp 1 issues, warps 2 to 5 are the epilogue, a thread per token.  Outputs whose rows begin on
+// multiples of 16 bytes leave through two 16 KB buffers and TMA stores (or reduce-adds: y += v never reads y); others
+// are written by the threads.
+constexpr int kOutBytes = BM * 128;  // 128 tokens x 128 bytes
+
+template <int BF>
+struct TileCfg {
+  static constexpr int kXBytes = BM * KB, kWBytes = BF * KB;
+  static constexpr int kStageBytes = kXBytes + kWBytes;
+  static constexpr int kStagesRaw = (196 * 1024) / kStageBytes;
+  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 2 * kOutBytes + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int kTmemCols = 2 * BF;
+  static_assert(kSmemBytes + BF * 4 + 64 <= 227 * 1024, "shared memory of a block");
+};
+
+// 16 bytes at column piece c of a row of 128 bytes, where a 128-byte swizzle puts them: the threads of a warp, a row
+// each, then write to different banks
+__device__ __forceinline__ void put16(uint32_t row_smem, int row, int c, uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+               ::"r"(row_smem + (uint32_t)((c ^ (row & 7)) << 4)), "r"(a), "r"(b), "r"(d), "r"(e) : "memory");
+}
+
+template <int MODE, int BF>
+__global__ void __launch_bounds__(kThreads, 1)
+q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ CUtensorMap map_y, const Args a, int by_tma, int n_t_tiles, int n_tiles) {
+  using C = TileCfg<BF>;
+  constexpr int kStages = C::kStages;
+  constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ __align__(16) float ws[BF];  // the scales of the tile's columns
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t out_smem = base + kStages * C::kStageBytes;
+  const uint32_t bars = out_smem + 2 * kOutBytes;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kStages + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kStages + 2 + b); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int total_kb = (a.K + KB - 1) / KB;
+  const int G = (int)gridDim.x, me = (int)blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), 4);  // one arrival per epilogue warp
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_slot)), "r"((uint32_t)C::kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_base_slot;
+  allow_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      grid_dependency_wait();
+      uint32_t armed = 0, armed_parity = 0;
+      int kbg = 0;
+      bool ok = true;
+      for (int tile = me; ok && tile < n_tiles; tile += G) {
+        const int f_tile = tile / n_t_tiles, t_tile = tile % n_t_tiles;
+        const int row0 = f_tile * kTileOutputs;
+        const int row1 = MODE == kGluBf16 ? a.N + row0 : row0 + BF / 2;
+        for (int kb = 0; kb < total_kb; ++kb, ++kbg) {
+          const int s = kbg % kStages;
+          const uint32_t phase = (kbg / kStages) & 1;
+          if (!mbar_wait(empty_bar(s), phase ^ 1, &abort_flag, a.error_flag, 1)) { ok = false; break; }
+          const uint32_t sx = base + s * C::kStageBytes, sw = sx + C::kXBytes;
+          mbar_expect_tx(full_bar(s), C::kStageBytes);
+          tma_load_2d(sx, &map_x, full_bar(s), kb * KB, t_tile * BM);
+          tma_load_2d(sw, &map_w, full_bar(s), kb * KB, row0);
+          tma_load_2d(sw + C::kWBytes / 2, &map_w, full_bar(s), kb * KB, row1);
+          armed |= 1u << s;
+          armed_parity = (armed_parity & ~(1u << s)) | (phase << s);
+        }
+      }
+      if (!ok)  // gave up: let the loads already issued land before the block's memory goes away
+        for (int s = 0; s < kStages; ++s)
+          if (armed & (1u << s)) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(full_bar(s), (armed_parity >> s) & 1) && clock64() - t0 < kWaitCycles) {}
+          }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_i8(BF);
+      int kbg = 0, it = 0;
+      bool ok = true;
+      for (int tile = me; ok && tile < n_tiles; tile += G, ++it) {
+        const int buf = it & 1;
+        // the epilogue must have drained this accumulator (two tiles ago)
+        if (!mbar_wait(acc_empty_bar(buf), ((it >> 1) & 1) ^ 1, &abort_flag, a.error_flag, 5)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem_base + buf * BF;
+        for (int kb = 0; kb < total_kb; ++kb, ++kbg) {
+          const int s = kbg % kStages;
+          const uint32_t phase = (kbg / kStages) & 1;
+          if (!mbar_wait(full_bar(s), phase, &abort_flag, a.error_flag, 2)) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t sx = base + s * C::kStageBytes;
+          const uint64_t dx = umma_desc(sx), dw = umma_desc(sx + C::kXBytes);
+#pragma unroll
+          for (int k = 0; k < KB / 32; ++k) umma_i8(d, dx + 2 * k, dw + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit(empty_bar(s));
+        }
+        umma_commit(acc_full_bar(buf));
+      }
+    }
+  } else {
+    grid_dependency_wait();
+    const int quad = warp & 3, row = quad * 32 + lane, et = threadIdx.x - 64;
+    const bool sender = warp == 2 && lane == 0;
+    int n_sent = 0, it = 0;
+    for (int tile = me; tile < n_tiles; tile += G, ++it) {
+      const int buf = it & 1;
+      const int f_tile = tile / n_t_tiles, t_tile = tile % n_t_tiles;
+      const int tok = t_tile * BM + row, f0 = f_tile * kTileOutputs;
+      const bool valid = tok < a.M;
+      const float xs = valid ? a.x_scale[tok] : 0.f;
+      asm volatile("barrier.sync 1, 128;" ::: "memory");  // the last tile's scales have been read
+      for (int c = et; c < BF; c += 128) {
+        const int f = MODE == kGluBf16 ? f0 + c % (BF / 2) : f0 + c;
+        ws[c] = f < a.N ? a.w_scale[MODE == kGluBf16 && c >= BF / 2 ? a.N + f : f] : 0.f;
+      }
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
+      if (!mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t taddr = tmem_base + buf * BF + ((uint32_t)(quad * 32) << 16);
+      // 32 columns at a time: values of this thread's token
+      auto values = [&](int c0, float* v) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld16(taddr + c0, r);
+        tmem_ld16(taddr + c0 + 16, r + 16);
+        if (MODE == kGluBf16) {
+          uint32_t u[32];
+          tmem_ld16(taddr + BF / 2 + c0, u);
+          tmem_ld16(taddr + BF / 2 + c0 + 16, u + 16);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            v[j] = silu_times(scaled((int)r[j], xs, ws[c0 + j]), scaled((int)u[j], xs, ws[BF / 2 + c0 + j]));
+        } else {
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = scaled((int)r[j], xs, ws[c0 + j]);
+        }
+      };
+      constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
+      if (by_tma) {
+        constexpr int kCols = f32 ? 32 : 64;  // outputs of a buffer's 128-byte rows
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTileOutputs; c0 += kCols) {
+          if (f0 + c0 >= a.N) break;  // the same for all four warps
+          const uint32_t out = out_smem + (uint32_t)(n_sent & 1) * kOutBytes;
+          // the send that read this buffer last (two sends ago) must be done with it
+          if (sender) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          asm volatile("barrier.sync 1, 128;" ::: "memory");
+          const uint32_t row_smem = out + (uint32_t)row * 128u;
+#pragma unroll
+          for (int h = 0; h < (f32 ? 1 : 2); ++h) {
+            float v[32];
+            values(c0 + 32 * h, v);
+            if (f32) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                put16(row_smem, row, c, __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]),
+                      __float_as_uint(v[4 * c + 3]));
+            } else {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                put16(row_smem, row, 4 * h + c, pack_bf16(v[8 * c], v[8 * c + 1]), pack_bf16(v[8 * c + 2], v[8 * c + 3]),
+                      pack_bf16(v[8 * c + 4], v[8 * c + 5]), pack_bf16(v[8 * c + 6], v[8 * c + 7]));
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the TMA unit reads what the threads wrote
+          asm volatile("barrier.sync 1, 128;" ::: "memory");
+          if (sender) {
+            if (MODE == kAccumF32)
+              asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(t_tile * BM) : "memory");
+            else
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(t_tile * BM) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          ++n_sent;
+        }
+      } else {
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTileOutputs; c0 += 32) {
+          if (f0 + c0 >= a.N) break;
+          float v[32];
+          values(c0, v);
+          if (!valid) continue;
+          const int n = min(32, a.N - f0 - c0);
+          const int64_t at = (int64_t)tok * a.ldy + f0 + c0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (j >= n) break;
+            if (f32) ((float*)a.y)[at + j] = MODE == kAccumF32 ? __fadd_rn(((const float*)a.y)[at + j], v[j]) : v[j];
+            else ((__nv_bfloat16*)a.y)[at + j] = __float2bfloat16_rn(v[j]);
+          }
+        }
+      }
+      // this warp has read its lanes of the accumulator: hand it back to the MMA warp
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty_bar(buf));
+    }
+    if (by_tma && sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the buffers go away with the block
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0) {  // every accumulator must be idle before its columns are freed
+      const int my_tiles = me < n_tiles ? (n_tiles - me + G - 1) / G : 0;
+      for (int b = 0; b < 2; ++b) {
+        const int uses = (my_tiles + 1 - b) / 2;  // tiles that used accumulator b
+        if (uses > 0) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(acc_full_bar(b), (uses - 1) & 1) && clock64() - t0 < kWaitCycles) {}
+        }
+      }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)C::kTmemCols) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------- host
+struct Operands {
+  const void* x; int64_t ldx;
+  const void* w; int64_t ldw; int w_rows;
+};
+
+int encode(CUtensorMap* m, CUtensorMapDataType type, int dims, const void* ptr, const cuuint64_t* size, const cuuint64_t* stride,
+           const cuuint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(kLaunchFailed, "linear_q8: the driver does not offer cuTensorMapEncodeTiled");
+  const cuuint32_t ones[3] = {1, 1, 1};
+  CUresult r = fn(m, type, dims, const_cast<void*>(ptr), size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? kOk : fail(kLaunchFailed, "linear_q8: cuTensorMapEncodeTiled failed with %d", (int)r);
+}
+// 8-bit rows [rows, K]: boxes of box_rows rows x one K block, or, K in whole blocks, x kkb K blocks one after the other
+int rows_map(CUtensorMap* m, const void* ptr, int64_t ld, int rows, int K, int box_rows, int kkb) {
+  if (kkb > 1) {
+    const cuuint64_t size[3] = {KB, (cuuint64_t)rows, (cuuint64_t)(K / KB)};
+    const cuuint64_t stride[2] = {(cuuint64_t)ld, KB};
+    const cuuint32_t box[3] = {KB, (cuuint32_t)box_rows, (cuuint32_t)kkb};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, ptr, size, stride, box);
+  }
+  const cuuint64_t size[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t stride[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {KB, (cuuint32_t)box_rows};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, ptr, size, stride, box);
+}
+
+constexpr int kMaxDevices = 64;
+int current_device() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+int sm_count() {
+  static int n[kMaxDevices] = {};
+  const int dev = current_device();
+  if (n[dev] == 0) {
+    int v = 0;
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    n[dev] = v > 0 ? v : 148;
+  }
+  return n[dev];
+}
+// Shared memory of a kernel, reserved once per device.
+template <typename K>
+int reserve(K kernel, int bytes, bool* done) {
+  const int dev = current_device();
+  if (done[dev]) return kOk;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(kLaunchFailed, "linear_q8: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+  done[dev] = true;
+  return kOk;
+}
+
+struct RowsPlan { int rows, splits, kkb, kstack; };
+
+// How many clusters of `size` blocks run at a time (one block per SM, clusters inside a GPC).
+int cluster_room(int size) {
+  static int room[kMaxDevices][2] = {};
+  const int dev = current_device();
+  int& n = room[dev][size == 4];
+  if (n == 0) {
+    auto kernel = q8_rows_kernel<64, kAccumF32, kCluster>;
+    static bool done[kMaxDevices] = {};
+    n = -1;
+    if (reserve(kernel, kRowsSmemBytes, done) != kOk) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024, 1, size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kRowsSmemBytes - 4096;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = size;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int v = 0;
+    if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) == cudaSuccess && v > 0) n = v;
+    else cudaGetLastError();
+  }
+  return n > 0 ? n : 0;
+}
+
+// The tile height is the smallest multiple of 8 whose tiles fill the SMs in whole waves.  Up to 16 tokens, tiles of at
+// most 64 rows stack 128 / rows K blocks into one MMA; a box brings about 32 KB of weights.  From 17 tokens on a product
+// that is not gated is cut along K into a cluster of 2 or 4, tiles as tall as lets all clusters run at once, whichever
+// moves fewer bytes per block (its share of the weight and of the tokens' rows).
+RowsPlan plan_rows(int N, int K, bool gated, int bn, bool fours) {
+  const int sms = sm_count();
+  const int n_kb = (K + KB - 1) / KB;
+  const bool whole = K % KB == 0;  // boxes of several K blocks
+  const int waves = (N + sms * 128 - 1) / (sms * 128);
+  int rows = (N + sms * waves - 1) / (sms * waves);
+  rows = (rows + 7) / 8 * 8;
+  rows = rows < 8 ? 8 : rows > 128 ? 128 : rows;
+  RowsPlan best{rows, 1, 1, 1};
+  if (!gated && bn > 16 && fours) {
+    long long best_cost = 0;
+    for (int splits = 2; splits <= 4; splits += 2) {
+      const int room = cluster_room(splits);
+      if (n_kb < 4 * splits || room < 1) continue;
+      int r = (N + room - 1) / room;
+      r = (r + 7) / 8 * 8;
+      if (r > 128) continue;
+      const int share = (n_kb + splits - 1) / splits;
+      const long long cost = (long long)(r + bn) * share;
+      if (best.splits == 1 || cost < best_cost) {
+        // boxes of two K blocks, unless whole boxes would leave the last split without one; the widest token tile's
+        // landing zone leaves the ring room for one
+        const bool pairs = whole && bn <= 64 && (splits - 1) * ((share + 1) / 2 * 2) < n_kb;
+        best = RowsPlan{r, splits, pairs ? 2 : 1, 1};
+        best_cost = cost;
+      }
+    }
+    if (best.splits > 1) return best;
+  }
+  if (!whole) return best;
+  if (gated || bn > 16) {
+    best.kkb = bn <= 64 && n_kb > 1 ? 2 : 1;
+    return best;
+  }
+  int kstack = 128 / rows;
+  if (kstack > 256 / bn) kstack = 256 / bn;
+  if (kstack > n_kb) kstack = n_kb;
+  const int group = kstack * rows * KB;  // bytes of weights that one MMA takes
+  int per_box = (28 * 1024 + group - 1) / group;
+  if (per_box > 16 / kstack) per_box = 16 / kstack;
+  if (per_box > (n_kb + kstack - 1) / kstack) per_box = (n_kb + kstack - 1) / kstack;
+  if (per_box < 1) per_box = 1;
+  while (per_box > 1 && per_box * kstack * (rows + bn) * KB > 48 * 1024) --per_box;
+  best.kkb = per_box * kstack;
+  best.kstack = kstack;
+  return best;
+}
+
+template <int BN, int MODE>
+int launch_rows(const Operands& o, const Args& a, cudaStream_t stream) {
+  constexpr bool gated = MODE == kGluBf16;
+  constexpr int kATiles = gated ? 2 : 1;
+  constexpr int M2 = gated ? kStoreBf16 : MODE;  // (no gated instance of the cluster and stacked kernels is built)
+  // the owners of a cluster write four neighbouring outputs of a token at once
+  const bool fours = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (MODE == kStoreBf16 ? 8 : 16) == 0;
+  const RowsPlan p = plan_rows(a.N, a.K, gated, BN, fours);
+  CUtensorMap mw, mx;
+  if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, p.rows, p.kkb)) return rc;
+  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BN, p.kkb)) return rc;
+  RowsArgs ra;
+  ra.rows_per_block = p.rows;
+  ra.kkb = p.kkb;
+  ra.kstack = p.kstack;
+  const int total_kb = (a.K + KB - 1) / KB;
+  ra.kb_per_split = ((total_kb + p.splits - 1) / p.splits + p.kkb - 1) / p.kkb * p.kkb;  // whole boxes
+  ra.tmem_cols = 32;
+  while (ra.tmem_cols < kATiles * p.kstack * BN) ra.tmem_cols *= 2;
+  const int stage = p.kkb * (kATiles * p.rows + BN) * KB;
+  // behind the ring: the cluster's landing zone or the stacked sums, at least what the MMA, reading 128 rows whatever
+  // the tile's height is, may run into
+  int landing = 0;
+  if (p.splits > 1) landing = ((BN + p.splits - 1) / p.splits * p.splits + 4) * BM * 4;
+  if (p.kstack > 1) landing = p.kstack * BN * p.rows * 4;
+  const int over_read = (BM - p.kstack * p.rows) * KB;
+  if (landing < over_read) landing = over_read;
+  const int fixed = 16 + 8 * (2 * kRowsMaxStages + 3) + 1024 + landing;
+  ra.n_stages = (kRowsSmemBytes - fixed) / stage;
+  if (ra.n_stages > kRowsMaxStages) ra.n_stages = kRowsMaxStages;
+  if (ra.n_stages < 2) return fail(kBadArgument, "linear_q8: stages of %d bytes do not fit twice", stage);
+  if (p.splits > 1 && ra.n_stages * stage < landing)  // the splits' tiles wait in the idle ring for their bulk copies
+    return fail(kBadArgument, "linear_q8: a ring of %d bytes is too small for the K splits' tiles", ra.n_stages * stage);
+  if (p.splits > 1 && (p.splits - 1) * ra.kb_per_split >= total_kb)
+    return fail(kBadArgument, "linear_q8: %d splits leave one without K blocks", p.splits);
+  const int smem = fixed + ra.n_stages * stage;
+  const dim3 grid((unsigned)((a.N + p.rows - 1) / p.rows), 1, (unsigned)p.splits);
+  if (p.splits > 1) {
+    static bool done[kMaxDevices] = {};
+    auto kernel = q8_rows_kernel<BN, M2, kCluster>;
+    if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
+    launch_overlapped_cluster(kernel, grid, dim3(kThreads), (size_t)smem, stream, (unsigned)p.splits, mw, mx, a, ra);
+  } else if (p.kstack > 1) {
+    static bool done[kMaxDevices] = {};
+    auto kernel = q8_rows_kernel<16, M2, kStacked>;
+    if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
+    launch_overlapped(kernel, grid, dim3(kThreads), (size_t)smem, stream, mw, mx, a, ra);
+  } else {
+    static bool done[kMaxDevices] = {};
+    auto kernel = q8_rows_kernel<BN, MODE, kPlain>;
+    if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
+    launch_overlapped(kernel, grid, dim3(kThreads), (size_t)smem, stream, mw, mx, a, ra);
+  }
+  return check_launch("linear_q8");
+}
+
+template <int MODE, int BF>
+int launch_tiles(const Operands& o, const Args& a, cudaStream_t stream) {
+  using C = TileCfg<BF>;
+  constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
+  constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
+  const int n_t = (a.M + BM - 1) / BM, n_f = (a.N + kTileOutputs - 1) / kTileOutputs;
+  const long long tiles = (long long)n_t * n_f;
+  if (tiles > 0x7fffffffLL) return fail(kBadArgument, "linear_q8: too many tiles");
+  CUtensorMap mx, mw, my;
+  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, 1)) return rc;
+  if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, BF / 2, 1)) return rc;
+  const int size = f32 ? 4 : 2;
+  // (a TMA store clips at whole 16-byte pieces: a row that ends inside one would write beyond it)
+  const bool by_tma = (uintptr_t)a.y % 16 == 0 && a.ldy * size % 16 == 0 && (int64_t)a.N * size % 16 == 0;
+  my = mx;  // not used unless by_tma; a valid map all the same
+  if (by_tma) {
+    const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
+    const cuuint64_t stride[1] = {(cuuint64_t)a.ldy * size};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), BM};
+    if (int rc = encode(&my, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, stride, box)) return rc;
+  }
+  static bool done[kMaxDevices] = {};
+  auto kernel = q8_tile_kernel<MODE, BF>;
+  if (int rc = reserve(kernel, C::kSmemBytes, done)) return rc;
+  const int sms = sm_count();
+  launch_overlapped(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kThreads), (size_t)C::kSmemBytes, stream, mx, mw, my, a,
+                    by_tma ? 1 : 0, n_t, (int)tiles);
+  return check_launch("linear_q8");
+}
+
+template <int MODE>
+int launch(const Operands& o, const Args& a, cudaStream_t stream) {
+  if (a.M <= 16) return launch_rows<16, MODE>(o, a, stream);
+  if (a.M <= 32) return launch_rows<32, MODE>(o, a, stream);
+  if (a.M <= 64) return launch_rows<64, MODE>(o, a, stream);
+  if (a.M <= 128) return launch_rows<128, MODE>(o, a, stream);
+  return launch_tiles<MODE, 256>(o, a, stream);
+}
+}  // namespace
+
+// x [M, K] and w [N (2N gated: the gate rows, then the up rows), K], rows that begin on multiples of 16 bytes.
+// mode 0: y = v (bfloat16), 1: y = v (float32), 2: y += v (float32), 3: y = silu(gate) * up (bfloat16).
+// The weight and its scales are read before the launch ahead in the stream has ended.
+extern "C" int skyla_linear_q8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw, const float* w_scale,
+                               int M, int N, int K, void* y, int64_t ldy, int mode, int* error_flag, cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return kOk;
+  if (K <= 0 || K > kMaxWidth) return fail(kBadArgument, "linear_q8: K=%d is outside 1..%d", K, kMaxWidth);
+  if (mode < kStoreBf16 || mode > kGluBf16) return fail(kBadArgument, "linear_q8: unknown mode %d", mode);
+  if (N > (1 << 30)) return fail(kBadArgument, "linear_q8: %d outputs", N);
+  if ((uintptr_t)x % 16 || (uintptr_t)w % 16 || ldx % 16 || ldw % 16)
+    return fail(kBadArgument, "linear_q8: rows that do not begin on multiples of 16 bytes");
+  const Operands o{x, ldx, w, ldw, mode == kGluBf16 ? 2 * N : N};
+  const Args a{y, ldy, M, N, K, x_scale, w_scale, error_flag};
+  switch (mode) {
+    case kStoreBf16: return launch<kStoreBf16>(o, a, stream);
+    case kStoreF32: return launch<kStoreF32>(o, a, stream);
+    case kAccumF32: return launch<kAccumF32>(o, a, stream);
+    default: return launch<kGluBf16>(o, a, stream);
+  }
+}

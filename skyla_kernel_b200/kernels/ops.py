@@ -776,6 +776,17 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
     _written(ldy, y, "linear_q8")
     dev = _device_of(x.q, x.scale, w.rows.q, w.rows.scale, y)
+    if m == 1:
+        ldx = w.ld  # the distance to a next row that is not there
+    if ldx % 16 == 0 and ldx >= k and x.q.data_ptr() % 16 == 0:
+        epilogue = {STORE: TC_STORE_F32 if code == F32 else TC_STORE_BF16, ACCUMULATE: TC_ACCUM_F32, GATED: TC_GLU_BF16}[mode]
+        f = _fn("gemm_q8", "skyla_linear_q8",
+                [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_int,
+                 c_void_p, c_void_p])
+        _launch_on(dev, "gemm_q8", f, x.q.data_ptr(), ldx, x.scale.data_ptr(), w.rows.q.data_ptr(), w.ld,
+                   w.rows.scale.data_ptr(), m, w.n_out, k, y.data_ptr(), ldy, epilogue,
+                   _state(state, y).error_flag.data_ptr())
+        return y
     f = _fn("linear_q8_plain", "skyla_linear_q8_plain",
             [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int64, c_int,
              c_void_p])
