@@ -41,31 +41,35 @@ __device__ __noinline__ int round_close(float x, float most, float z) {
   return x < 0.f ? -n : n;
 }
 // z = x * inv is within 127 * 2^-23 < 2^-15 of the exact quotient (two roundings), so its nearest integer is
-// the exact quotient's unless z lies within 2^-15 of a half.
-__device__ __forceinline__ int round_q(float x, const Step& s) {
-  const float z = x * s.inv;
-  const float n = rintf(z);
-  if (fabsf(z - n) > 0.5f - 0x1p-15f) return round_close(x, s.most, z);
-  return (int)n;
+// the exact quotient's unless z lies within 2^-15 of a half.  Adding 1.5 * 2^23 rounds z to an integer (to even)
+// and leaves it in the low bits.
+template <int E>
+__device__ __forceinline__ void round_q(const float* x, const Step& s, uint32_t* n) {
+  constexpr float kMagic = 12582912.f;
+  bool close = false;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const float z = x[i] * s.inv, m = z + kMagic;
+    n[i] = __float_as_uint(m);
+    close |= fabsf(z - (m - kMagic)) > 0.5f - 0x1p-15f;
+  }
+  if (close) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float z = x[i] * s.inv;
+      if (fabsf(z - rintf(z)) > 0.5f - 0x1p-15f) n[i] = (uint32_t)round_close(x[i], s.most, z);
+    }
+  }
+}
+// the low bytes of four words
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t* n) {
+  return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
 }
 
 // A product's sum with its two scales, in one order and never contracted into an addition that follows: every
 // kernel of the 8-bit product gives the same bits.
 __device__ __forceinline__ float scaled(int acc, float x_scale, float w_scale) {
   return __fmul_rn(__fmul_rn(__int2float_rn(acc), x_scale), w_scale);
-}
-
-// Largest of a block's values, given to every thread; `scratch` holds 32 words.
-__device__ __forceinline__ unsigned block_max(unsigned v, unsigned* scratch) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n_warps = (blockDim.x + 31) >> 5;
-  v = __reduce_max_sync(0xffffffffu, v);
-  __syncthreads();
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  unsigned m = 0;
-  for (int i = 0; i < n_warps; ++i) m = max(m, scratch[i]);
-  return m;
 }
 
 }  // namespace q8

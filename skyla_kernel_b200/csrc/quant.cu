@@ -1,80 +1,289 @@
 // Rows in 8 bits (q8.cuh): quantised from bfloat16 or 32-bit values, from a root-mean-square norm, and back.
+// All three are bound by the memory.  A row belongs to one group of threads (a warp for short rows, else a block), which
+// reads it once, 16 bytes a thread and load, keeps it in registers while the group agrees on the row's largest value
+// (one reduction), and writes its integers.  Elements beyond what the registers hold (kKeep loads a thread) are read again.
+// Rows that do not begin on multiples of 16 bytes, or whose width leaves part of a load, go element by element.
 #include "q8.cuh"
 using namespace skyla;
 using namespace skyla::q8;
 SKYLA_EXPORT_ERROR_MESSAGE()
 
 namespace {
+constexpr int kNormThreads = 512;  // most threads of a norm's block: they hold 32-bit products, twice what a row's bfloat16 takes
 
-template <typename TI>
-__global__ void quantize_kernel(const TI* __restrict__ x, int64_t ldx, int width, int8_t* __restrict__ q, int64_t ldq,
-                                float* __restrict__ scale) {
-  __shared__ unsigned scratch[32];
+template <int BYTES> struct Word;
+template <> struct Word<1> { typedef uint8_t type; };
+template <> struct Word<2> { typedef uint16_t type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<16> { typedef uint4 type; };
+
+// E neighbouring elements, in loads and stores of at most 16 bytes
+template <typename T, int E>
+struct Pack {
+  static constexpr int kBytes = E * (int)sizeof(T), kPiece = kBytes < 16 ? kBytes : 16, kPieces = kBytes / kPiece;
+  typedef typename Word<kPiece>::type W;
+  union { W w[kPieces]; uint16_t h[kBytes / 2 > 0 ? kBytes / 2 : 1]; uint32_t u[kBytes / 4 > 0 ? kBytes / 4 : 1]; };
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) w[i] = reinterpret_cast<const W*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<W*>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if (sizeof(T) == 4) return __uint_as_float(u[i]);
+    return __uint_as_float((uint32_t)h[i] << 16);  // a bfloat16 is the upper half of a 32-bit value
+  }
+  __device__ __forceinline__ void set(int i, float v) {
+    if (sizeof(T) == 4) u[i] = __float_as_uint(v);
+    else h[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  }
+};
+
+template <int E>
+__device__ __forceinline__ void store_q(int8_t* p, const uint32_t* n) {
+  if constexpr (E == 1) *p = (int8_t)n[0];
+  else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = low_bytes(n);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(low_bytes(n), low_bytes(n + 4));
+}
+
+// The threads of a row: `BLOCK` a block's, else a warp's
+template <bool BLOCK>
+struct Group {
+  int64_t row; int rank, size;
+  __device__ __forceinline__ Group() {
+    if (BLOCK) { row = blockIdx.x; rank = threadIdx.x; size = blockDim.x; }
+    else { row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); rank = threadIdx.x & 31; size = 32; }
+  }
+  // largest of the group's words and sum of its values, both with one meeting; the sum's order is fixed by the group
+  __device__ __forceinline__ void meet(unsigned& most, float* sum) const {
+    __shared__ unsigned tops[32];
+    __shared__ float sums[32];
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (sum != nullptr) *sum = warp_sum(*sum);
+    if (!BLOCK) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    if (lane == 0) {
+      tops[warp] = most;
+      if (sum != nullptr) sums[warp] = *sum;
+    }
+    __syncthreads();
+    most = __reduce_max_sync(0xffffffffu, lane < n_warps ? tops[lane] : 0u);
+    if (sum != nullptr) *sum = warp_sum(lane < n_warps ? sums[lane] : 0.f);
+  }
+};
+
+template <typename T, int E, int kKeep, bool BLOCK>
+__global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t n_rows, int width, int8_t* __restrict__ q,
+                                int64_t ldq, float* __restrict__ scale) {
   allow_dependents();
   grid_dependency_wait();
-  const int64_t r = blockIdx.x;
-  const TI* xr = x + r * ldx;
-  unsigned m = 0;
-  for (int i = threadIdx.x; i < width; i += blockDim.x) m = max(m, abs_bits(to_float(xr[i])));
-  m = block_max(m, scratch);
-  const bool bad = m >= kInfBits;
-  const Step s = step_of(bad ? 0u : m);
-  for (int i = threadIdx.x; i < width; i += blockDim.x) q[r * ldq + i] = bad ? 0 : (int8_t)round_q(to_float(xr[i]), s);
-  if (threadIdx.x == 0) scale[r] = bad ? kNan : s.most / kMost;
+  const Group<BLOCK> g;
+  if (g.row >= n_rows) return;  // (whole warps: a block has one row only)
+  const T* xr = x + g.row * ldx;
+  int8_t* qr = q + g.row * ldq;
+  const int first = g.rank * E, step = g.size * E;
+  Pack<T, E> kept[kKeep];
+  unsigned most = 0;
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (first + j * step < width) kept[j].load(xr + first + j * step);
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (first + j * step < width) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) most = max(most, abs_bits(kept[j].get(i)));
+    }
+  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
+    Pack<T, E> p;
+    p.load(xr + e);
+#pragma unroll
+    for (int i = 0; i < E; ++i) most = max(most, abs_bits(p.get(i)));
+  }
+  g.meet(most, nullptr);
+  const bool bad = most >= kInfBits;
+  const Step s = step_of(bad ? 0u : most);
+  auto put = [&](int64_t e, const Pack<T, E>& p) {
+    float v[E];
+    uint32_t n[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = bad ? 0.f : p.get(i);
+    round_q<E>(v, s, n);
+    store_q<E>(qr + e, n);
+  };
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (first + j * step < width) put(first + j * step, kept[j]);
+  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
+    Pack<T, E> p;
+    p.load(xr + e);
+    put(e, p);
+  }
+  if (g.rank == 0) scale[g.row] = bad ? kNan : s.most / kMost;
 }
 
 // x += residual (rounded to x's type: the norm is that of the sum as it is kept), then the norm's row in 8 bits.
 // With t = x * w the norm is t * inv, inv = 1 / sqrt(mean(x^2) + eps) one number for the row, and 127 t inv / (A inv)
-// = 127 t / A: the integers do not depend on inv, which goes into the scale alone.
-template <typename TX, typename TR, bool ADD>
-__global__ void rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int width,
-                                  const float* __restrict__ w, float eps, int8_t* __restrict__ q, int64_t ldq,
+// = 127 t / A: the integers do not depend on inv, which goes into the scale alone, so the sum of squares and the largest
+// t are found in one pass and one meeting.
+template <typename TX, typename TR, bool ADD, int E, int kKeep, bool BLOCK>
+__global__ void __launch_bounds__(kNormThreads) rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int64_t n_rows,
+                                  int width, const float* __restrict__ w, float eps, int8_t* __restrict__ q, int64_t ldq,
                                   float* __restrict__ scale) {
-  __shared__ unsigned scratch[32];
-  __shared__ float fscratch[32];
   allow_dependents();
   grid_dependency_wait();
-  const int64_t r = blockIdx.x;
-  TX* xr = x + r * ldx;
+  const Group<BLOCK> g;
+  if (g.row >= n_rows) return;
+  TX* xr = x + g.row * ldx;
+  const TR* rr = ADD ? residual + g.row * ldr : nullptr;
+  int8_t* qr = q + g.row * ldq;
+  const int first = g.rank * E, step = g.size * E;
   float ss = 0.f;
-  unsigned m = 0;
-  for (int i = threadIdx.x; i < width; i += blockDim.x) {
-    float v = to_float(xr[i]);
+  unsigned most = 0;
+  // t of E elements, the sum written back
+  auto take = [&](int64_t e, Pack<TX, E>& p, const Pack<TR, E>& add, const Pack<float, E>& weight, float* t) {
     if (ADD) {
-      const TX kept = from_float<TX>(v + to_float(residual[r * ldr + i]));
-      xr[i] = kept;
-      v = to_float(kept);
+#pragma unroll
+      for (int i = 0; i < E; ++i) p.set(i, p.get(i) + add.get(i));
+      p.store(xr + e);
     }
-    ss = fmaf(v, v, ss);
-    m = max(m, abs_bits(v * w[i]));
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float v = p.get(i);
+      ss = fmaf(v, v, ss);
+      t[i] = v * weight.get(i);
+      most = max(most, abs_bits(t[i]));
+    }
+  };
+  float kept[kKeep][E];
+  {
+    Pack<TX, E> p[kKeep];
+    Pack<TR, E> add[kKeep];
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (first + j * step < width) {
+        p[j].load(xr + first + j * step);
+        if (ADD) add[j].load(rr + first + j * step);
+      }
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (first + j * step < width) {
+        Pack<float, E> weight;
+        weight.load(w + first + j * step);
+        take(first + j * step, p[j], add[j], weight, kept[j]);
+      }
   }
-  m = block_max(m, scratch);
-  ss = block_sum(ss, fscratch);
+  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
+    Pack<TX, E> p;
+    Pack<TR, E> add;
+    Pack<float, E> weight;
+    p.load(xr + e);
+    if (ADD) add.load(rr + e);
+    weight.load(w + e);
+    float t[E];
+    take(e, p, add, weight, t);
+  }
+  g.meet(most, &ss);
   const float inv = 1.0f / sqrtf(ss / (float)width + eps);
-  const bool bad = m >= kInfBits || abs_bits(ss) >= kInfBits || abs_bits(inv) >= kInfBits;
-  const Step s = step_of(bad ? 0u : m);
-  for (int i = threadIdx.x; i < width; i += blockDim.x)
-    q[r * ldq + i] = bad ? 0 : (int8_t)round_q(to_float(xr[i]) * w[i], s);
-  if (threadIdx.x == 0) scale[r] = bad ? kNan : s.most * inv / kMost;
+  const bool bad = most >= kInfBits || abs_bits(ss) >= kInfBits || abs_bits(inv) >= kInfBits;
+  const Step s = step_of(bad ? 0u : most);
+  auto put = [&](int64_t e, const float* t) {
+    float v[E];
+    uint32_t n[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = bad ? 0.f : t[i];
+    round_q<E>(v, s, n);
+    store_q<E>(qr + e, n);
+  };
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (first + j * step < width) put(first + j * step, kept[j]);
+  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {  // (this thread wrote these sums itself)
+    Pack<TX, E> p;
+    Pack<float, E> weight;
+    p.load(xr + e);
+    weight.load(w + e);
+    float t[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) t[i] = p.get(i) * weight.get(i);
+    put(e, t);
+  }
+  if (g.rank == 0) scale[g.row] = bad ? kNan : s.most * inv / kMost;
 }
 
-template <typename TO>
-__global__ void dequantize_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int width,
-                                  TO* __restrict__ out, int64_t ldo) {
+template <typename T, int E, bool BLOCK>
+__global__ void __launch_bounds__(1024) dequantize_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale, int64_t n_rows,
+                                  int width, T* __restrict__ out, int64_t ldo) {
   allow_dependents();
   grid_dependency_wait();
-  const int64_t r = blockIdx.x;
-  const float s = scale[r];
-  for (int i = threadIdx.x; i < width; i += blockDim.x) out[r * ldo + i] = from_float<TO>((float)q[r * ldq + i] * s);
+  const Group<BLOCK> g;
+  if (g.row >= n_rows) return;
+  const int8_t* qr = q + g.row * ldq;
+  T* o = out + g.row * ldo;
+  const float s = scale[g.row];
+  auto put = [&](int64_t e, const typename Word<E>::type& raw) {
+    const int8_t* n = reinterpret_cast<const int8_t*>(&raw);
+    Pack<T, E> p;
+#pragma unroll
+    for (int i = 0; i < E; ++i) p.set(i, (float)n[i] * s);
+    p.store(o + e);
+  };
+  int64_t e = (int64_t)g.rank * E;
+  const int64_t step = (int64_t)g.size * E;
+  for (; e + 3 * step < width; e += 4 * step) {  // four loads in flight
+    typename Word<E>::type raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const typename Word<E>::type*>(qr + e + j * step);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put(e + j * step, raw[j]);
+  }
+  for (; e < width; e += step) put(e, *reinterpret_cast<const typename Word<E>::type*>(qr + e));
 }
-
-int threads_for(int width) { return width >= 2048 ? 512 : (width >= 512 ? 256 : 128); }
 
 int check_sizes(const char* what, int64_t n_rows, int width, int64_t ld_in, int64_t ld_out) {
   if (width <= 0) return fail(kBadArgument, "%s: rows of %d", what, width);
   if (n_rows > 0x7fffffffLL) return fail(kBadArgument, "%s: more than 2^31 - 1 rows", what);
-  if (ld_out < width || ld_in < 0) return fail(kBadArgument, "%s: row strides do not fit rows of %d", what, width);
+  if (ld_out < 0 || ld_in < 0) return fail(kBadArgument, "%s: row strides do not fit rows of %d", what, width);
   return kOk;
+}
+// Rows of `size`-byte elements that begin on multiples of `bytes`
+bool rows_on(const void* p, int64_t ld, int size, int bytes) { return (uintptr_t)p % bytes == 0 && ld * size % bytes == 0; }
+
+// How a row is shared out: threads, and loads that each keeps.
+struct Shape { int threads; int keep; bool block; };
+Shape shape_for(int64_t n_rows, int width, int E, int most = 1024) {
+  const int64_t loads = ((int64_t)width + E - 1) / E;
+  // a warp a row, eight rows a block
+  if (loads <= 32 * 4 && n_rows >= 8) return {256, loads <= 32 ? 1 : 4, false};
+  // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last
+  int64_t threads = n_rows < 592 ? loads : (loads + 3) / 4;
+  threads = (threads + 31) / 32 * 32;
+  if (threads < 64) threads = 64;
+  if (threads > most) threads = most;
+  return {(int)threads, loads <= threads ? 1 : 4, true};
+}
+dim3 grid_for(int64_t n_rows, const Shape& s) { return dim3((unsigned)(s.block ? n_rows : (n_rows + s.threads / 32 - 1) / (s.threads / 32))); }
+
+template <typename T, int E>
+void launch_quantize(const Shape& s, const void* x, int64_t ldx, int64_t n_rows, int width, void* q, int64_t ldq, float* scale,
+                     cudaStream_t stream) {
+  auto go = [&](auto kernel) {
+    launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const T*)x, ldx, n_rows, width, (int8_t*)q, ldq, scale);
+  };
+  if (s.block) s.keep == 1 ? go(quantize_kernel<T, E, 1, true>) : go(quantize_kernel<T, E, 4, true>);
+  else s.keep == 1 ? go(quantize_kernel<T, E, 1, false>) : go(quantize_kernel<T, E, 4, false>);
+}
+template <typename TX, typename TR, bool ADD, int E>
+void launch_norm(const Shape& s, void* x, int64_t ldx, const void* residual, int64_t ldr, int64_t n_rows, int width, const float* w,
+                 float eps, void* q, int64_t ldq, float* scale, cudaStream_t stream) {
+  auto go = [&](auto kernel) {
+    launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (TX*)x, ldx, (const TR*)residual, ldr, n_rows, width,
+                      w, eps, (int8_t*)q, ldq, scale);
+  };
+  if (s.block) s.keep == 1 ? go(rmsnorm_q8_kernel<TX, TR, ADD, E, 1, true>) : go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, true>);
+  else s.keep == 1 ? go(rmsnorm_q8_kernel<TX, TR, ADD, E, 1, false>) : go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, false>);
 }
 }  // namespace
 
@@ -82,9 +291,12 @@ extern "C" int skyla_quantize_rows(const void* x, int x_dtype, int64_t ldx, int6
                                    float* scale, cudaStream_t stream) {
   if (n_rows <= 0) return kOk;
   if (int rc = check_sizes("quantize_rows", n_rows, width, ldx, ldq)) return rc;
-  SKYLA_DISPATCH(x_dtype, TI, {
-    launch_overlapped(quantize_kernel<TI>, dim3((unsigned)n_rows), dim3(threads_for(width)), 0, stream, (const TI*)x, ldx,
-                      width, (int8_t*)q, ldq, scale);
+  SKYLA_DISPATCH(x_dtype, T, {
+    constexpr int E = 16 / sizeof(T);
+    if (width % E == 0 && rows_on(x, ldx, sizeof(T), 16) && rows_on(q, ldq, 1, E))
+      launch_quantize<T, E>(shape_for(n_rows, width, E), x, ldx, n_rows, width, q, ldq, scale, stream);
+    else
+      launch_quantize<T, 1>(shape_for(n_rows, width, 1), x, ldx, n_rows, width, q, ldq, scale, stream);
   });
   return check_launch("quantize_rows");
 }
@@ -95,18 +307,22 @@ extern "C" int skyla_rmsnorm_q8(void* x, int x_dtype, int64_t ldx, const void* r
   if (n_rows <= 0) return kOk;
   if (int rc = check_sizes("rmsnorm_q8", n_rows, width, ldx, ldq)) return rc;
   if (!(eps >= 0.f)) return fail(kBadArgument, "rmsnorm_q8: eps must not be negative");
-  const dim3 grid((unsigned)n_rows), block(threads_for(width));
-  if (residual == nullptr) {
-    SKYLA_DISPATCH(x_dtype, TX, {
-      launch_overlapped(rmsnorm_q8_kernel<TX, float, false>, grid, block, 0, stream, (TX*)x, ldx, (const float*)nullptr,
-                        (int64_t)0, width, weight, eps, (int8_t*)q, ldq, scale);
-    });
-  } else {
-    SKYLA_DISPATCH(x_dtype, TX, SKYLA_DISPATCH(r_dtype, TR, {
-      launch_overlapped(rmsnorm_q8_kernel<TX, TR, true>, grid, block, 0, stream, (TX*)x, ldx, (const TR*)residual, ldr, width,
-                        weight, eps, (int8_t*)q, ldq, scale);
-    }););
-  }
+  SKYLA_DISPATCH(x_dtype, TX, {
+    constexpr int E = 16 / sizeof(TX);
+    const int r_size = r_dtype == kF32 ? 4 : 2;
+    // (an element of a residual of another type than x's takes E * r_size bytes a load: 8, 16 or twice 16)
+    const bool vec = width % E == 0 && rows_on(x, ldx, sizeof(TX), 16) && rows_on(q, ldq, 1, E) && (uintptr_t)weight % 16 == 0 &&
+                     (residual == nullptr || rows_on(residual, ldr, r_size, E * r_size < 16 ? E * r_size : 16));
+    if (residual == nullptr) {
+      if (vec) launch_norm<TX, float, false, E>(shape_for(n_rows, width, E, kNormThreads), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
+      else launch_norm<TX, float, false, 1>(shape_for(n_rows, width, 1, kNormThreads), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
+    } else {
+      SKYLA_DISPATCH(r_dtype, TR, {
+        if (vec) launch_norm<TX, TR, true, E>(shape_for(n_rows, width, E, kNormThreads), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
+        else launch_norm<TX, TR, true, 1>(shape_for(n_rows, width, 1, kNormThreads), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
+      });
+    }
+  });
   return check_launch("rmsnorm_q8");
 }
 
@@ -114,9 +330,14 @@ extern "C" int skyla_dequantize_rows(const void* q, int64_t ldq, const float* sc
                                      int out_dtype, int64_t ldo, cudaStream_t stream) {
   if (n_rows <= 0) return kOk;
   if (int rc = check_sizes("dequantize_rows", n_rows, width, ldq, ldo)) return rc;
-  SKYLA_DISPATCH(out_dtype, TO, {
-    launch_overlapped(dequantize_kernel<TO>, dim3((unsigned)n_rows), dim3(threads_for(width)), 0, stream, (const int8_t*)q, ldq,
-                      scale, width, (TO*)out, ldo);
+  SKYLA_DISPATCH(out_dtype, T, {
+    auto go = [&](auto kernel, const Shape& s) {
+      launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const int8_t*)q, ldq, scale, n_rows, width, (T*)out, ldo);
+    };
+    const bool vec = width % 8 == 0 && rows_on(q, ldq, 1, 8) && rows_on(out, ldo, sizeof(T), 16);
+    const Shape s = shape_for(n_rows, width, vec ? 8 : 1);
+    if (vec) s.block ? go(dequantize_kernel<T, 8, true>, s) : go(dequantize_kernel<T, 8, false>, s);
+    else s.block ? go(dequantize_kernel<T, 1, true>, s) : go(dequantize_kernel<T, 1, false>, s);
   });
   return check_launch("dequantize_rows");
 }
