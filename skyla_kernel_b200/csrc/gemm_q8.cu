@@ -421,10 +421,14 @@ q8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // ---------------------------------------------------------------------------------- many tokens
 // One block per SM walks tiles of 128 tokens x BF accumulator columns (a gated weight: BF / 2 gate rows and the BF / 2
 // up rows of the same outputs), two accumulators in turn: the epilogue of one tile runs beside the products of the
-// next.  warp 0 loads, warp 1 issues, warps 2 to 5 are the epilogue, a thread per token.  Outputs whose rows begin on
-// multiples of 16 bytes leave through two 16 KB buffers and TMA stores (or reduce-adds: y += v never reads y); others
-// are written by the threads.
+// next.  warp 0 loads, warp 1 issues, warps 2 to 5 are the epilogue, a thread per token.  32 or 64 outputs of the tile's
+// tokens at a time are laid out in one of two 16 KB buffers and leave by a TMA store (or reduce-add: y += v never reads
+// y), or, where y's rows do not allow that, row by row in order.
+// SPLIT: few tiles; the blocks of a cluster share one tile, each with a run of its K blocks.  They leave their
+// accumulators in shared memory (the ring, idle by then), and each finishes an equal part of the columns from all of
+// them, read through distributed shared memory: whole numbers, so the result does not show the cut.
 constexpr int kOutBytes = BM * 128;  // 128 tokens x 128 bytes
+constexpr int kMaxSplits = 4;
 
 template <int BF>
 struct TileCfg {
@@ -435,6 +439,7 @@ struct TileCfg {
   static constexpr int kSmemBytes = kStages * kStageBytes + 2 * kOutBytes + 1024 /*align*/ + 256 /*barriers*/;
   static constexpr int kTmemCols = 2 * BF;
   static_assert(kSmemBytes + BF * 4 + 64 <= 227 * 1024, "shared memory of a block");
+  static_assert(kStages * kStageBytes >= BM * BF * 4, "a split's accumulator fits the ring");
 };
 
 // 16 bytes at column piece c of a row of 128 bytes, where a 128-byte swizzle puts them: the threads of a warp, a row
@@ -444,13 +449,20 @@ __device__ __forceinline__ void put16(uint32_t row_smem, int row, int c, uint32_
                ::"r"(row_smem + (uint32_t)((c ^ (row & 7)) << 4)), "r"(a), "r"(b), "r"(d), "r"(e) : "memory");
 }
 
-template <int MODE, int BF>
+struct TileArgs {
+  int by_tma;         // map_y is y's: outputs leave by TMA
+  int n_t_tiles, n_tiles;
+  int splits;         // blocks of a cluster (SPLIT), each with an equal run of the K blocks; else 1
+};
+
+template <int MODE, int BF, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-               const __grid_constant__ CUtensorMap map_y, const Args a, int by_tma, int n_t_tiles, int n_tiles) {
+               const __grid_constant__ CUtensorMap map_y, const Args a, const TileArgs ta) {
   using C = TileCfg<BF>;
   constexpr int kStages = C::kStages;
   constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
+  constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint32_t tmem_base_slot;
   __shared__ volatile int abort_flag;
@@ -464,7 +476,12 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kStages + 2 + b); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int total_kb = (a.K + KB - 1) / KB;
-  const int G = (int)gridDim.x, me = (int)blockIdx.x;
+  // the tiles of this block: first, first + step, ... ; a split's block has one
+  const int rank = SPLIT ? (int)blockIdx.x % ta.splits : 0;
+  const int first = SPLIT ? (int)blockIdx.x / ta.splits : (int)blockIdx.x;
+  const int step = SPLIT ? ta.n_tiles : (int)gridDim.x;
+  const int kb_lo = SPLIT ? rank * total_kb / ta.splits : 0;  // (at most 3 x 1,024)
+  const int kb_hi = SPLIT ? (rank + 1) * total_kb / ta.splits : total_kb;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -491,23 +508,33 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
   if (warp == 0) {
     if (lane == 0) {
-      grid_dependency_wait();
       uint32_t armed = 0, armed_parity = 0;
       int kbg = 0;
-      bool ok = true;
-      for (int tile = me; ok && tile < n_tiles; tile += G) {
-        const int f_tile = tile / n_t_tiles, t_tile = tile % n_t_tiles;
+      bool ok = true, waited = false;
+      for (int tile = first; ok && tile < ta.n_tiles; tile += step) {
+        const int f_tile = tile / ta.n_t_tiles, t_tile = tile % ta.n_t_tiles;
         const int row0 = f_tile * kTileOutputs;
         const int row1 = MODE == kGluBf16 ? a.N + row0 : row0 + BF / 2;
-        for (int kb = 0; kb < total_kb; ++kb, ++kbg) {
-          const int s = kbg % kStages;
-          const uint32_t phase = (kbg / kStages) & 1;
-          if (!mbar_wait(empty_bar(s), phase ^ 1, &abort_flag, a.error_flag, 1)) { ok = false; break; }
-          const uint32_t sx = base + s * C::kStageBytes, sw = sx + C::kXBytes;
+        auto load_weights = [&](int kb, int s) {
+          const uint32_t sw = base + s * C::kStageBytes + C::kXBytes;
           mbar_expect_tx(full_bar(s), C::kStageBytes);
-          tma_load_2d(sx, &map_x, full_bar(s), kb * KB, t_tile * BM);
           tma_load_2d(sw, &map_w, full_bar(s), kb * KB, row0);
           tma_load_2d(sw + C::kWBytes / 2, &map_w, full_bar(s), kb * KB, row1);
+        };
+        // weights are finished before any launch that reads them: the ring's first filling of them is asked for
+        // before this grid waits for the one ahead of it
+        const int n_pre = waited ? 0 : min(kStages, kb_hi - kb_lo);
+        for (int i = 0; i < n_pre; ++i) load_weights(kb_lo + i, i);
+        if (!waited) grid_dependency_wait();
+        waited = true;
+        for (int kb = kb_lo; kb < kb_hi; ++kb, ++kbg) {
+          const int s = kbg % kStages;
+          const uint32_t phase = (kbg / kStages) & 1;
+          if (kbg >= n_pre) {
+            if (!mbar_wait(empty_bar(s), phase ^ 1, &abort_flag, a.error_flag, 1)) { ok = false; break; }
+            load_weights(kb, s);
+          }
+          tma_load_2d(base + s * C::kStageBytes, &map_x, full_bar(s), kb * KB, t_tile * BM);
           armed |= 1u << s;
           armed_parity = (armed_parity & ~(1u << s)) | (phase << s);
         }
@@ -524,13 +551,13 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       const uint32_t idesc = idesc_i8(BF);
       int kbg = 0, it = 0;
       bool ok = true;
-      for (int tile = me; ok && tile < n_tiles; tile += G, ++it) {
+      for (int tile = first; ok && tile < ta.n_tiles; tile += step, ++it) {
         const int buf = it & 1;
         // the epilogue must have drained this accumulator (two tiles ago)
         if (!mbar_wait(acc_empty_bar(buf), ((it >> 1) & 1) ^ 1, &abort_flag, a.error_flag, 5)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem_base + buf * BF;
-        for (int kb = 0; kb < total_kb; ++kb, ++kbg) {
+        for (int kb = kb_lo; kb < kb_hi; ++kb, ++kbg) {
           const int s = kbg % kStages;
           const uint32_t phase = (kbg / kStages) & 1;
           if (!mbar_wait(full_bar(s), phase, &abort_flag, a.error_flag, 2)) { ok = false; break; }
@@ -538,121 +565,190 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           const uint32_t sx = base + s * C::kStageBytes;
           const uint64_t dx = umma_desc(sx), dw = umma_desc(sx + C::kXBytes);
 #pragma unroll
-          for (int k = 0; k < KB / 32; ++k) umma_i8(d, dx + 2 * k, dw + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < KB / 32; ++k) umma_i8(d, dx + 2 * k, dw + 2 * k, idesc, (kb > kb_lo || k > 0) ? 1u : 0u);
           umma_commit(empty_bar(s));
         }
         umma_commit(acc_full_bar(buf));
       }
     }
   } else {
-    grid_dependency_wait();
     const int quad = warp & 3, row = quad * 32 + lane, et = threadIdx.x - 64;
     const bool sender = warp == 2 && lane == 0;
     int n_sent = 0, it = 0;
-    for (int tile = me; tile < n_tiles; tile += G, ++it) {
+    bool waited = false;
+    for (int tile = first; tile < ta.n_tiles; tile += step, ++it) {
       const int buf = it & 1;
-      const int f_tile = tile / n_t_tiles, t_tile = tile % n_t_tiles;
-      const int tok = t_tile * BM + row, f0 = f_tile * kTileOutputs;
-      const bool valid = tok < a.M;
-      const float xs = valid ? a.x_scale[tok] : 0.f;
+      const int f_tile = tile / ta.n_t_tiles, t_tile = tile % ta.n_t_tiles;
+      const int tok0 = t_tile * BM, tok = tok0 + row, f0 = f_tile * kTileOutputs;
       asm volatile("barrier.sync 1, 128;" ::: "memory");  // the last tile's scales have been read
       for (int c = et; c < BF; c += 128) {
         const int f = MODE == kGluBf16 ? f0 + c % (BF / 2) : f0 + c;
         ws[c] = f < a.N ? a.w_scale[MODE == kGluBf16 && c >= BF / 2 ? a.N + f : f] : 0.f;
       }
+      if (!waited) grid_dependency_wait();
+      waited = true;
+      const float xs = tok < a.M ? a.x_scale[tok] : 0.f;
       asm volatile("barrier.sync 1, 128;" ::: "memory");
-      if (!mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3)) break;
+      bool ok = mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3);
+      if (!SPLIT && !ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_base + buf * BF + ((uint32_t)(quad * 32) << 16);
+      // the ring as a split leaves its accumulator there: [piece of four columns][row], a warp's rows 512 bytes in a row
+      const uint32_t left = base + 16u * (uint32_t)row;
+      if (SPLIT) {
+        if (ok) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < BF; c0 += 32) {
+            uint32_t r[32];
+            __syncwarp();
+            tmem_ld16(taddr + c0, r);
+            tmem_ld16(taddr + c0 + 16, r + 16);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                           ::"r"(left + (uint32_t)(c0 / 4 + c) * (BM * 16u)), "r"(r[4 * c]), "r"(r[4 * c + 1]), "r"(r[4 * c + 2]),
+                             "r"(r[4 * c + 3]) : "memory");
+          }
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      }
+      // 16 columns of this thread's token: the accumulator's, or the sum of all splits'
+      auto columns16 = [&](int c0, uint32_t* r) {
+        if (SPLIT) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = 0;
+#pragma unroll
+          for (int q = 0; q < kMaxSplits; ++q) {
+            if (q >= ta.splits) break;
+            uint32_t from;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(left + (uint32_t)(c0 / 4) * (BM * 16u)), "r"((uint32_t)q));
+            uint32_t v[16];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4 * c]), "=r"(v[4 * c + 1]), "=r"(v[4 * c + 2]),
+                           "=r"(v[4 * c + 3]) : "r"(from + (uint32_t)c * (BM * 16u)) : "memory");
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] += v[j];
+          }
+        } else {
+          tmem_ld16(taddr + c0, r);
+        }
+      };
       // 32 columns at a time: values of this thread's token
       auto values = [&](int c0, float* v) {
         uint32_t r[32];
         __syncwarp();
-        tmem_ld16(taddr + c0, r);
-        tmem_ld16(taddr + c0 + 16, r + 16);
+        columns16(c0, r);
+        columns16(c0 + 16, r + 16);
         if (MODE == kGluBf16) {
           uint32_t u[32];
-          tmem_ld16(taddr + BF / 2 + c0, u);
-          tmem_ld16(taddr + BF / 2 + c0 + 16, u + 16);
-          tmem_wait_ld();
+          columns16(BF / 2 + c0, u);
+          columns16(BF / 2 + c0 + 16, u + 16);
+          if (!SPLIT) tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             v[j] = silu_times(scaled((int)r[j], xs, ws[c0 + j]), scaled((int)u[j], xs, ws[BF / 2 + c0 + j]));
         } else {
-          tmem_wait_ld();
+          if (!SPLIT) tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = scaled((int)r[j], xs, ws[c0 + j]);
         }
       };
-      constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
-      if (by_tma) {
-        constexpr int kCols = f32 ? 32 : 64;  // outputs of a buffer's 128-byte rows
+      constexpr int kCols = f32 ? 32 : (kTileOutputs < 64 ? kTileOutputs : 64);  // outputs of a buffer's rows
+      constexpr int kChunks = kTileOutputs / kCols;
+      // a split's block finishes every ta.splits-th chunk
 #pragma unroll 1
-        for (int c0 = 0; c0 < kTileOutputs; c0 += kCols) {
-          if (f0 + c0 >= a.N) break;  // the same for all four warps
-          const uint32_t out = out_smem + (uint32_t)(n_sent & 1) * kOutBytes;
-          // the send that read this buffer last (two sends ago) must be done with it
-          if (sender) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          asm volatile("barrier.sync 1, 128;" ::: "memory");
-          const uint32_t row_smem = out + (uint32_t)row * 128u;
+      for (int chunk = rank; chunk < kChunks; chunk += SPLIT ? ta.splits : 1) {
+        const int c0 = chunk * kCols;
+        if (f0 + c0 >= a.N) break;  // the same for all four warps
+        const uint32_t out = out_smem + (uint32_t)(n_sent & 1) * kOutBytes;
+        // who read this buffer last (two chunks ago) must be done with it: the send, or, row by row, the warps, which
+        // have met since
+        if (ta.by_tma && sender) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        asm volatile("barrier.sync 1, 128;" ::: "memory");
+        const uint32_t row_smem = out + (uint32_t)row * 128u;
 #pragma unroll
-          for (int h = 0; h < (f32 ? 1 : 2); ++h) {
-            float v[32];
-            values(c0 + 32 * h, v);
-            if (f32) {
+        for (int h = 0; h < kCols / 32; ++h) {
+          float v[32];
+          values(c0 + 32 * h, v);
+          if (f32) {
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                put16(row_smem, row, c, __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]),
-                      __float_as_uint(v[4 * c + 3]));
-            } else {
+            for (int c = 0; c < 8; ++c)
+              put16(row_smem, row, c, __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]),
+                    __float_as_uint(v[4 * c + 3]));
+          } else {
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
-                put16(row_smem, row, 4 * h + c, pack_bf16(v[8 * c], v[8 * c + 1]), pack_bf16(v[8 * c + 2], v[8 * c + 3]),
-                      pack_bf16(v[8 * c + 4], v[8 * c + 5]), pack_bf16(v[8 * c + 6], v[8 * c + 7]));
-            }
+            for (int c = 0; c < 4; ++c)
+              put16(row_smem, row, 4 * h + c, pack_bf16(v[8 * c], v[8 * c + 1]), pack_bf16(v[8 * c + 2], v[8 * c + 3]),
+                    pack_bf16(v[8 * c + 4], v[8 * c + 5]), pack_bf16(v[8 * c + 6], v[8 * c + 7]));
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the TMA unit reads what the threads wrote
-          asm volatile("barrier.sync 1, 128;" ::: "memory");
-          if (sender) {
+        }
+        if (ta.by_tma) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the TMA unit reads what the threads wrote
+        asm volatile("barrier.sync 1, 128;" ::: "memory");
+        if (ta.by_tma) {
+          if (sender && (!SPLIT || !abort_flag)) {
             if (MODE == kAccumF32)
               asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
-                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(t_tile * BM) : "memory");
+                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(tok0) : "memory");
             else
               asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
-                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(t_tile * BM) : "memory");
+                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(tok0) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-          ++n_sent;
-        }
-      } else {
-#pragma unroll 1
-        for (int c0 = 0; c0 < kTileOutputs; c0 += 32) {
-          if (f0 + c0 >= a.N) break;
-          float v[32];
-          values(c0, v);
-          if (!valid) continue;
-          const int n = min(32, a.N - f0 - c0);
-          const int64_t at = (int64_t)tok * a.ldy + f0 + c0;
+        } else {
+          // a warp takes 32 rows, one after the other, its lanes neighbouring outputs
+#pragma unroll 4
+          for (int i = 0; i < 32; ++i) {
+            const int r = quad * 32 + i;
+            if (tok0 + r >= a.M) break;
+            const int64_t at = (int64_t)(tok0 + r) * a.ldy + f0 + c0;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j >= n) break;
-            if (f32) ((float*)a.y)[at + j] = MODE == kAccumF32 ? __fadd_rn(((const float*)a.y)[at + j], v[j]) : v[j];
-            else ((__nv_bfloat16*)a.y)[at + j] = __float2bfloat16_rn(v[j]);
+            for (int h = 0; h < kCols / 32; ++h) {
+              const int c = lane + 32 * h;
+              const uint32_t from = out + (uint32_t)r * 128u +
+                                    (uint32_t)((((c * (f32 ? 4 : 2)) >> 4) ^ (r & 7)) << 4) + (uint32_t)((c * (f32 ? 4 : 2)) & 15);
+              if (f0 + c0 + c >= a.N) continue;
+              if (f32) {
+                float v;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+                float* y = (float*)a.y + at + c;
+                *y = MODE == kAccumF32 ? __fadd_rn(*y, v) : v;
+              } else {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+                ((uint16_t*)a.y)[at + c] = v;
+              }
+            }
           }
         }
+        ++n_sent;
       }
       // this warp has read its lanes of the accumulator: hand it back to the MMA warp
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty_bar(buf));
     }
-    if (by_tma && sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the buffers go away with the block
+    if (ta.by_tma && sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the buffers go away with the block
+  }
+  if (SPLIT) {
+    // two meetings of all threads of the cluster: every accumulator lies in its ring; all have read them.  (The
+    // epilogue's warps took the first one above.)
+    if (warp < 2) {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1) {
     if (lane == 0) {  // every accumulator must be idle before its columns are freed
-      const int my_tiles = me < n_tiles ? (n_tiles - me + G - 1) / G : 0;
+      const int my_tiles = first < ta.n_tiles ? (ta.n_tiles - first + step - 1) / step : 0;
       for (int b = 0; b < 2; ++b) {
         const int uses = (my_tiles + 1 - b) / 2;  // tiles that used accumulator b
         if (uses > 0) {
@@ -861,34 +957,85 @@ int launch_rows(const Operands& o, const Args& a, cudaStream_t stream) {
   return check_launch("linear_q8");
 }
 
-template <int MODE, int BF>
-int launch_tiles(const Operands& o, const Args& a, cudaStream_t stream) {
+// How a product of many tokens is cut: the accumulator's columns and the splits of K, whichever is done first by what
+// was measured of one: a K block's time, what a tile costs beside its K blocks, a cluster's two meetings (nanoseconds).
+struct TilePlan { int columns, splits; };
+TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
+  const long long n_kb = (K + KB - 1) / KB, n_t = (M + BM - 1) / BM;
+  TilePlan best{256, 1};
+  double best_ns = 0;
+  for (int columns = 64; columns <= 256; columns *= 2) {
+    if (gated && columns == 64) continue;
+    const double per_kb = columns == 256 ? 450.0 : columns == 128 ? 280.0 : 200.0;
+    const double per_tile = columns == 256 ? 2200 : columns == 128 ? 1300 : 900;
+    const int outputs = gated ? columns / 2 : columns;
+    const long long tiles = n_t * ((N + outputs - 1) / outputs);
+    for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
+      if (splits > 1 && (tiles > cluster_room(splits) || n_kb < 2 * splits)) break;
+      const long long waves = (tiles * splits + sms - 1) / sms, kbs = (n_kb + splits - 1) / splits;
+      // the epilogue of all but a block's last tile runs beside the next tile's products
+      const double main = (double)kbs * per_kb;
+      const double ns = (double)(waves - 1) * (main > per_tile ? main : per_tile) + main + per_tile / splits + (splits > 1 ? 1500 : 0);
+      if (best_ns == 0 || ns < best_ns) { best = TilePlan{columns, splits}; best_ns = ns; }
+    }
+  }
+  return best;
+}
+
+template <int MODE, int BF, bool SPLIT>
+int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stream) {
   using C = TileCfg<BF>;
   constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
   constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
-  const int n_t = (a.M + BM - 1) / BM, n_f = (a.N + kTileOutputs - 1) / kTileOutputs;
-  const long long tiles = (long long)n_t * n_f;
-  if (tiles > 0x7fffffffLL) return fail(kBadArgument, "linear_q8: too many tiles");
+  TileArgs ta;
+  ta.n_t_tiles = (a.M + BM - 1) / BM;
+  const long long tiles = (long long)ta.n_t_tiles * ((a.N + kTileOutputs - 1) / kTileOutputs);
+  if (tiles > 0x3fffffffLL) return fail(kBadArgument, "linear_q8: too many tiles");
+  ta.n_tiles = (int)tiles;
   CUtensorMap mx, mw, my;
   if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, 1)) return rc;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, BF / 2, 1)) return rc;
   const int size = f32 ? 4 : 2;
   // (a TMA store clips at whole 16-byte pieces: a row that ends inside one would write beyond it)
-  const bool by_tma = (uintptr_t)a.y % 16 == 0 && a.ldy * size % 16 == 0 && (int64_t)a.N * size % 16 == 0;
+  ta.by_tma = (uintptr_t)a.y % 16 == 0 && a.ldy * size % 16 == 0 && (int64_t)a.N * size % 16 == 0;
   my = mx;  // not used unless by_tma; a valid map all the same
-  if (by_tma) {
+  if (ta.by_tma) {
     const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
     const cuuint64_t stride[1] = {(cuuint64_t)a.ldy * size};
     const cuuint32_t box[2] = {(cuuint32_t)(128 / size), BM};
     if (int rc = encode(&my, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, stride, box)) return rc;
   }
   static bool done[kMaxDevices] = {};
-  auto kernel = q8_tile_kernel<MODE, BF>;
+  auto kernel = q8_tile_kernel<MODE, BF, SPLIT>;
   if (int rc = reserve(kernel, C::kSmemBytes, done)) return rc;
   const int sms = sm_count();
-  launch_overlapped(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kThreads), (size_t)C::kSmemBytes, stream, mx, mw, my, a,
-                    by_tma ? 1 : 0, n_t, (int)tiles);
+  ta.splits = SPLIT ? splits : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(SPLIT ? (unsigned)(tiles * splits) : (unsigned)(tiles < sms ? tiles : sms));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (SPLIT) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (overlap_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kernel, mx, mw, my, a, ta);
   return check_launch("linear_q8");
+}
+template <int MODE, int BF>
+int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stream) {
+  return splits > 1 ? launch_tiles<MODE, BF, true>(o, a, splits, stream) : launch_tiles<MODE, BF, false>(o, a, 1, stream);
 }
 
 template <int MODE>
@@ -897,7 +1044,10 @@ int launch(const Operands& o, const Args& a, cudaStream_t stream) {
   if (a.M <= 32) return launch_rows<32, MODE>(o, a, stream);
   if (a.M <= 64) return launch_rows<64, MODE>(o, a, stream);
   if (a.M <= 128) return launch_rows<128, MODE>(o, a, stream);
-  return launch_tiles<MODE, 256>(o, a, stream);
+  const TilePlan p = plan_tiles(a.M, a.N, a.K, MODE == kGluBf16, sm_count());
+  if (p.columns == 256) return launch_tiles<MODE, 256>(o, a, p.splits, stream);
+  if (p.columns == 64 && MODE != kGluBf16) return launch_tiles<MODE == kGluBf16 ? kStoreBf16 : MODE, 64>(o, a, p.splits, stream);
+  return launch_tiles<MODE, 128>(o, a, p.splits, stream);
 }
 }  // namespace
 
