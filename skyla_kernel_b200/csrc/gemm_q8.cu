@@ -221,7 +221,7 @@ q8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const float ws = mine ? a.w_scale[f] : 0.f;
     const float us = MODE == kGluBf16 && mine ? a.w_scale[a.N + f] : 0.f;
     grid_dependency_wait();
-    if (et < BN) tok_scale[et] = et < a.M ? a.x_scale[et] : 0.f;
+    for (int t = et; t < BN; t += 128) tok_scale[t] = t < a.M ? a.x_scale[t] : 0.f;
     const int kstack = stacked ? ra.kstack : 1;
     int* red = reinterpret_cast<int*>(smem_raw + (landing - smem_u32(smem_raw)));
     float old_pre[4] = {0.f, 0.f, 0.f, 0.f}, old16[16];
@@ -430,12 +430,16 @@ q8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 constexpr int kOutBytes = BM * 128;  // 128 tokens x 128 bytes
 constexpr int kMaxSplits = 4;
 
-template <int BF>
+template <int MODE, int BF>
 struct TileCfg {
-  static constexpr int kXBytes = BM * KB, kWBytes = BF * KB;
-  static constexpr int kStageBytes = kXBytes + kWBytes;
+  // K blocks of a stage.  (A TMA load takes its unit about 0.1 us whatever it brings: narrow tiles bring two a load.
+  // A gated tile's gate and up rows come by loads of their own and have to lie together for one instruction of BF
+  // columns: one K block a stage.  Two, with instructions of half the width: 416 against 344 us for 4,096 tokens.)
+  static constexpr int kKkb = BF == 256 || MODE == kGluBf16 ? 1 : 2;
+  static constexpr int kXBytes = BM * KB, kWBytes = BF * KB;  // of one K block
+  static constexpr int kStageBytes = kKkb * (kXBytes + kWBytes);
   static constexpr int kStagesRaw = (196 * 1024) / kStageBytes;
-  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
+  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;  // 4, 3, 4
   static constexpr int kSmemBytes = kStages * kStageBytes + 2 * kOutBytes + 1024 /*align*/ + 256 /*barriers*/;
   static constexpr int kTmemCols = 2 * BF;
   static_assert(kSmemBytes + BF * 4 + 64 <= 227 * 1024, "shared memory of a block");
@@ -451,6 +455,7 @@ __device__ __forceinline__ void put16(uint32_t row_smem, int row, int c, uint32_
 
 struct TileArgs {
   int by_tma;         // map_y is y's: outputs leave by TMA
+  int boxes;          // the maps of x and w bring a stage's K blocks at once (K in whole blocks); else one by one
   int n_t_tiles, n_tiles;
   int splits;         // blocks of a cluster (SPLIT), each with an equal run of the K blocks; else 1
 };
@@ -459,7 +464,7 @@ template <int MODE, int BF, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                const __grid_constant__ CUtensorMap map_y, const Args a, const TileArgs ta) {
-  using C = TileCfg<BF>;
+  using C = TileCfg<MODE, BF>;
   constexpr int kStages = C::kStages;
   constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
   constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
@@ -506,35 +511,53 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   const uint32_t tmem_base = tmem_base_slot;
   allow_dependents();
 
+  constexpr int kKkb = C::kKkb;
+  const int n_st = (kb_hi - kb_lo + kKkb - 1) / kKkb;  // stages of a tile
+
   if (warp == 0) {
     if (lane == 0) {
       uint32_t armed = 0, armed_parity = 0;
-      int kbg = 0;
+      int stg = 0;
       bool ok = true, waited = false;
       for (int tile = first; ok && tile < ta.n_tiles; tile += step) {
         const int f_tile = tile / ta.n_t_tiles, t_tile = tile % ta.n_t_tiles;
         const int row0 = f_tile * kTileOutputs;
-        const int row1 = MODE == kGluBf16 ? a.N + row0 : row0 + BF / 2;
-        auto load_weights = [&](int kb, int s) {
-          const uint32_t sw = base + s * C::kStageBytes + C::kXBytes;
+        // (blocks past the end of K, or of this split, are loaded as what lies there, zeros past the end, and not used)
+        auto load_weights = [&](int i, int s) {
+          const int kb = kb_lo + i * kKkb;
+          const uint32_t sw = base + s * C::kStageBytes + kKkb * C::kXBytes;
           mbar_expect_tx(full_bar(s), C::kStageBytes);
-          tma_load_2d(sw, &map_w, full_bar(s), kb * KB, row0);
-          tma_load_2d(sw + C::kWBytes / 2, &map_w, full_bar(s), kb * KB, row1);
+          if (MODE == kGluBf16) {
+            tma_load_2d(sw, &map_w, full_bar(s), kb * KB, row0);
+            tma_load_2d(sw + C::kWBytes / 2, &map_w, full_bar(s), kb * KB, a.N + row0);
+          } else if (kKkb > 1 && ta.boxes) {
+            tma_load_3d(sw, &map_w, full_bar(s), 0, row0, kb);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kKkb; ++j) tma_load_2d(sw + j * C::kWBytes, &map_w, full_bar(s), (kb + j) * KB, row0);
+          }
         };
         // weights are finished before any launch that reads them: the ring's first filling of them is asked for
         // before this grid waits for the one ahead of it
-        const int n_pre = waited ? 0 : min(kStages, kb_hi - kb_lo);
-        for (int i = 0; i < n_pre; ++i) load_weights(kb_lo + i, i);
+        const int n_pre = waited ? 0 : min(kStages, n_st);
+        for (int i = 0; i < n_pre; ++i) load_weights(i, i);
         if (!waited) grid_dependency_wait();
         waited = true;
-        for (int kb = kb_lo; kb < kb_hi; ++kb, ++kbg) {
-          const int s = kbg % kStages;
-          const uint32_t phase = (kbg / kStages) & 1;
-          if (kbg >= n_pre) {
+        for (int i = 0; i < n_st; ++i, ++stg) {
+          const int s = stg % kStages;
+          const uint32_t phase = (stg / kStages) & 1;
+          if (stg >= n_pre) {
             if (!mbar_wait(empty_bar(s), phase ^ 1, &abort_flag, a.error_flag, 1)) { ok = false; break; }
-            load_weights(kb, s);
+            load_weights(i, s);
           }
-          tma_load_2d(base + s * C::kStageBytes, &map_x, full_bar(s), kb * KB, t_tile * BM);
+          const uint32_t sx = base + s * C::kStageBytes;
+          const int kb = kb_lo + i * kKkb;
+          if (kKkb > 1 && ta.boxes) {
+            tma_load_3d(sx, &map_x, full_bar(s), 0, t_tile * BM, kb);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kKkb; ++j) tma_load_2d(sx + j * C::kXBytes, &map_x, full_bar(s), (kb + j) * KB, t_tile * BM);
+          }
           armed |= 1u << s;
           armed_parity = (armed_parity & ~(1u << s)) | (phase << s);
         }
@@ -549,7 +572,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = idesc_i8(BF);
-      int kbg = 0, it = 0;
+      int stg = 0, it = 0;
       bool ok = true;
       for (int tile = first; ok && tile < ta.n_tiles; tile += step, ++it) {
         const int buf = it & 1;
@@ -557,15 +580,23 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         if (!mbar_wait(acc_empty_bar(buf), ((it >> 1) & 1) ^ 1, &abort_flag, a.error_flag, 5)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem_base + buf * BF;
-        for (int kb = kb_lo; kb < kb_hi; ++kb, ++kbg) {
-          const int s = kbg % kStages;
-          const uint32_t phase = (kbg / kStages) & 1;
+        uint32_t started = 0;
+        for (int i = 0; i < n_st; ++i, ++stg) {
+          const int s = stg % kStages;
+          const uint32_t phase = (stg / kStages) & 1;
           if (!mbar_wait(full_bar(s), phase, &abort_flag, a.error_flag, 2)) { ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t sx = base + s * C::kStageBytes;
-          const uint64_t dx = umma_desc(sx), dw = umma_desc(sx + C::kXBytes);
+          const uint32_t sx = base + s * C::kStageBytes, sw = sx + kKkb * C::kXBytes;
 #pragma unroll
-          for (int k = 0; k < KB / 32; ++k) umma_i8(d, dx + 2 * k, dw + 2 * k, idesc, (kb > kb_lo || k > 0) ? 1u : 0u);
+          for (int j = 0; j < kKkb; ++j) {
+            if (kb_lo + i * kKkb + j >= kb_hi) break;
+            const uint64_t dx = umma_desc(sx + j * C::kXBytes), dw = umma_desc(sw + j * C::kWBytes);
+#pragma unroll
+            for (int k = 0; k < KB / 32; ++k) {
+              umma_i8(d, dx + 2 * k, dw + 2 * k, idesc, started);
+              started = 1u;
+            }
+          }
           umma_commit(empty_bar(s));
         }
         umma_commit(acc_full_bar(buf));
@@ -617,21 +648,23 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       // 16 columns of this thread's token: the accumulator's, or the sum of all splits'
       auto columns16 = [&](int c0, uint32_t* r) {
         if (SPLIT) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = 0;
+          uint32_t v[kMaxSplits][16];  // the loads of all splits are in flight together
 #pragma unroll
           for (int q = 0; q < kMaxSplits; ++q) {
-            if (q >= ta.splits) break;
+            if (q >= ta.splits) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[q][j] = 0;
+              continue;
+            }
             uint32_t from;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(left + (uint32_t)(c0 / 4) * (BM * 16u)), "r"((uint32_t)q));
-            uint32_t v[16];
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4 * c]), "=r"(v[4 * c + 1]), "=r"(v[4 * c + 2]),
-                           "=r"(v[4 * c + 3]) : "r"(from + (uint32_t)c * (BM * 16u)) : "memory");
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] += v[j];
+              asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[q][4 * c]), "=r"(v[q][4 * c + 1]),
+                           "=r"(v[q][4 * c + 2]), "=r"(v[q][4 * c + 3]) : "r"(from + (uint32_t)c * (BM * 16u)) : "memory");
           }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = v[0][j] + v[1][j] + v[2][j] + v[3][j];
         } else {
           tmem_ld16(taddr + c0, r);
         }
@@ -698,7 +731,9 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
-          // a warp takes 32 rows, one after the other, its lanes neighbouring outputs
+          // a warp takes 32 rows, one after the other, its lanes neighbouring outputs.  (Compact code: a launch starts
+          // with cold instruction caches.  Eight rows at a time, pairs of bfloat16 in one store: 333 tokens x 2,561 to
+          // 1,111 took 10.4 instead of 8.7 us.)
 #pragma unroll 4
           for (int i = 0; i < 32; ++i) {
             const int r = quad * 32 + i;
@@ -958,25 +993,30 @@ int launch_rows(const Operands& o, const Args& a, cudaStream_t stream) {
 }
 
 // How a product of many tokens is cut: the accumulator's columns and the splits of K, whichever is done first by what
-// was measured of one: a K block's time, what a tile costs beside its K blocks, a cluster's two meetings (nanoseconds).
+// was measured (nanoseconds, 4,096 inputs at 130 to 2,048 tokens): a K block takes 370 / 245 / 205 at 256 / 128 / 64
+// columns, what a tile costs beside its K blocks is 5,200 / 3,450 / 2,800, a cluster's two meetings and the exchange
+// 3,500 (two blocks) or 4,700.  (A gated product of 200 tokens by the weight-streaming kernel, two instructions of 256
+// columns for 32 bytes of K: 39 against 30 us.)
 struct TilePlan { int columns, splits; };
 TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
   const long long n_kb = (K + KB - 1) / KB, n_t = (M + BM - 1) / BM;
   TilePlan best{256, 1};
   double best_ns = 0;
+  auto offer = [&](int columns, int splits, double ns) {
+    if (best_ns == 0 || ns < best_ns) { best = TilePlan{columns, splits}; best_ns = ns; }
+  };
   for (int columns = 64; columns <= 256; columns *= 2) {
     if (gated && columns == 64) continue;
-    const double per_kb = columns == 256 ? 450.0 : columns == 128 ? 280.0 : 200.0;
-    const double per_tile = columns == 256 ? 2200 : columns == 128 ? 1300 : 900;
+    const double per_kb = columns == 256 ? 370 : columns == 128 ? 245 : 205;
+    const double beside = columns == 256 ? 5200 : columns == 128 ? 3450 : 2800;
     const int outputs = gated ? columns / 2 : columns;
     const long long tiles = n_t * ((N + outputs - 1) / outputs);
     for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
       if (splits > 1 && (tiles > cluster_room(splits) || n_kb < 2 * splits)) break;
-      const long long waves = (tiles * splits + sms - 1) / sms, kbs = (n_kb + splits - 1) / splits;
-      // the epilogue of all but a block's last tile runs beside the next tile's products
-      const double main = (double)kbs * per_kb;
-      const double ns = (double)(waves - 1) * (main > per_tile ? main : per_tile) + main + per_tile / splits + (splits > 1 ? 1500 : 0);
-      if (best_ns == 0 || ns < best_ns) { best = TilePlan{columns, splits}; best_ns = ns; }
+      const long long waves = (tiles * splits + sms - 1) / sms;
+      double main = (double)((n_kb + splits - 1) / splits) * per_kb;
+      if (waves > 1 && main < beside / 2) main = beside / 2;  // (the epilogue of all but the last tile runs beside the next)
+      offer(columns, splits, (double)waves * main + beside + (splits == 2 ? 3500 : splits == 4 ? 4700 : 0));
     }
   }
   return best;
@@ -984,7 +1024,7 @@ TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
 
 template <int MODE, int BF, bool SPLIT>
 int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stream) {
-  using C = TileCfg<BF>;
+  using C = TileCfg<MODE, BF>;
   constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
   constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
   TileArgs ta;
@@ -993,8 +1033,10 @@ int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stre
   if (tiles > 0x3fffffffLL) return fail(kBadArgument, "linear_q8: too many tiles");
   ta.n_tiles = (int)tiles;
   CUtensorMap mx, mw, my;
-  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, 1)) return rc;
-  if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, BF / 2, 1)) return rc;
+  ta.boxes = C::kKkb > 1 && a.K % KB == 0;
+  const int kkb = ta.boxes ? C::kKkb : 1;
+  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, kkb)) return rc;
+  if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, MODE == kGluBf16 ? BF / 2 : BF, kkb)) return rc;
   const int size = f32 ? 4 : 2;
   // (a TMA store clips at whole 16-byte pieces: a row that ends inside one would write beyond it)
   ta.by_tma = (uintptr_t)a.y % 16 == 0 && a.ldy * size % 16 == 0 && (int64_t)a.N * size % 16 == 0;
