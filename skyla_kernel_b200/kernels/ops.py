@@ -250,7 +250,7 @@ def default_state(device) -> KernelState:
 
 
 def _state(state: Optional[KernelState], t: torch.Tensor) -> KernelState:
-    return state if state is not None else default_state(t.device)
+    return state if state is not None else _DEFAULT_STATES.get(t.device) or default_state(t.device)
 
 
 def check_device_errors(device) -> None:
@@ -608,42 +608,76 @@ def q8_rows(n: int, width: int, device) -> Q8Rows:
     return Q8Rows(q if q.shape[1] == width else q[:, :width], torch.empty(n, dtype=torch.float32, device=device))
 
 
-def _q8(rows: Q8Rows, what: str) -> int:
-    """Row stride of 8-bit rows, after their check."""
+def _dims(t: torch.Tensor, what: str):
+    """(rows, width, row stride) of a 2-D tensor whose rows are contiguous."""
+    if t.dim() != 2:
+        raise KernelError(f"{what}: expected a 2-D tensor, got shape {tuple(t.shape)}")
+    n, width = t.shape
+    ld, step = t.stride()
+    if step != 1 and width > 1:
+        raise KernelError(f"{what}: expected contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
+    return n, width, ld if n > 1 else max(ld, width)
+
+
+def _written_dims(t: torch.Tensor, what: str):
+    """The same of a matrix that a kernel writes: its rows must not lie on one another."""
+    n, width, ld = _dims(t, what)
+    if ld < width:
+        raise KernelError(f"{what}: rows of {width} elements {ld} apart would be written over one another")
+    return n, width, ld
+
+
+def _q8_dims(rows: Q8Rows, what: str, dims=_dims):
+    """(rows, width, row stride) of 8-bit rows, after their check."""
     q, scale = rows
-    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+    if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise KernelError(f"{what}: 8-bit rows are int8 with float32 scales, not {q.dtype} and {scale.dtype}")
-    ld = _rows(q, what)
-    if scale.dim() != 1 or scale.shape[0] != q.shape[0] or not scale.is_contiguous():
+    n, width, ld = dims(q, what)
+    if scale.shape != (n,) or not scale.is_contiguous():
         raise KernelError(f"{what}: one contiguous scale per row, got {tuple(scale.shape)} for rows {tuple(q.shape)}")
-    return ld
-
-
-def _written(ld: int, t: torch.Tensor, what: str) -> int:
-    """The row stride of a matrix that a kernel writes: its rows must not lie on one another."""
-    if ld < t.shape[1] and t.shape[0] > 1:
-        raise KernelError(f"{what}: rows of {t.shape[1]} elements {ld} apart would be written over one another")
-    return ld
+    return n, width, ld
 
 
 def _device_of(*tensors) -> int:
     """The one CUDA device of the operands."""
     dev = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0 or not t.is_cuda:
             raise KernelError("kernel operands must be CUDA tensors; there is no host path")
-        if t.get_device() != dev:
-            raise KernelError(f"kernel operands on devices {dev} and {t.get_device()}")
+        if at != dev:
+            raise KernelError(f"kernel operands on devices {dev} and {at}")
     return dev
 
 
-def _launch_on(dev: int, module: str, f, *args) -> None:
-    """Launch on the operands' device, whichever is current, on its current stream."""
-    if dev == torch.cuda.current_device():
-        _check(module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
-    else:
-        with torch.cuda.device(dev):
-            _check(module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+class _Launcher:
+    """A kernel launcher whose last argument is the stream: called on its operands' device, whichever is current, on
+    that device's current stream."""
+
+    __slots__ = ("module", "name", "argtypes", "f")
+
+    def __init__(self, module: str, name: str, *argtypes):
+        self.module, self.name, self.argtypes, self.f = module, name, [*argtypes, c_void_p], None
+
+    def __call__(self, dev: int, *args) -> None:
+        f = self.f
+        if f is None:
+            f = self.f = _fn(self.module, self.name, self.argtypes)
+        if dev == torch._C._cuda_getDevice():
+            _check(self.module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+        else:
+            with torch.cuda.device(dev):
+                _check(self.module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+
+
+_quantize_rows = _Launcher("quant", "skyla_quantize_rows", c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p)
+_dequantize_rows = _Launcher("quant", "skyla_dequantize_rows", c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64)
+_rmsnorm_q8 = _Launcher("quant", "skyla_rmsnorm_q8", c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p,
+                        c_float, c_void_p, c_int64, c_void_p)
+_linear_q8 = _Launcher("gemm_q8", "skyla_linear_q8", c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int,
+                       c_void_p, c_int64, c_int, c_void_p)
+_linear_q8_plain = _Launcher("linear_q8_plain", "skyla_linear_q8_plain", c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                             c_int, c_int, c_int, c_void_p, c_int, c_int64, c_int)
 
 
 def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
@@ -651,31 +685,26 @@ def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
     ``q = x / scale``, the exact quotient rounded to the nearest integer (ties to even).
 
     A row of zeros stays zeros; a row that holds a NaN or an infinity gets the scale NaN and zeros."""
-    ld, code = _rows(x, "quantize_rows"), dtype_code(x)
-    n, width = x.shape
+    n, width, ld = _dims(x, "quantize_rows")
+    code = dtype_code(x)
     if out is None:
         out = q8_rows(n, width, x.device)
-    if out.q.shape != x.shape:
-        raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(out.q.shape)}")
-    ldq = _written(_q8(out, "quantize_rows"), out.q, "quantize_rows")
-    dev = _device_of(x, out.q, out.scale)
-    f = _fn("quant", "skyla_quantize_rows",
-            [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p])
-    _launch_on(dev, "quant", f, x.data_ptr(), code, ld, n, width, out.q.data_ptr(), ldq, out.scale.data_ptr())
+    q, scale = out
+    m, w, ldq = _q8_dims(out, "quantize_rows", _written_dims)
+    if m != n or w != width:
+        raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
+    _quantize_rows(_device_of(x, q, scale), x.data_ptr(), code, ld, n, width, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
 
 def dequantize_rows(rows: Q8Rows, out: torch.Tensor) -> torch.Tensor:
     """What 8-bit rows stand for: ``out[r] = q[r] * scale[r]`` in ``out``'s type (bfloat16 or float32)."""
-    ldq, ldo, code = _q8(rows, "dequantize_rows"), _rows(out, "dequantize_rows"), dtype_code(out)
-    if rows.q.shape != out.shape:
-        raise KernelError(f"dequantize_rows: rows {tuple(rows.q.shape)} do not go into {tuple(out.shape)}")
-    _written(ldo, out, "dequantize_rows")
-    dev = _device_of(rows.q, rows.scale, out)
-    f = _fn("quant", "skyla_dequantize_rows",
-            [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p])
-    _launch_on(dev, "quant", f, rows.q.data_ptr(), ldq, rows.scale.data_ptr(), out.shape[0], out.shape[1],
-               out.data_ptr(), code, ldo)
+    q, scale = rows
+    n, width, ldq = _q8_dims(rows, "dequantize_rows")
+    m, w, ldo = _written_dims(out, "dequantize_rows")
+    if m != n or w != width:
+        raise KernelError(f"dequantize_rows: rows {tuple(q.shape)} do not go into {tuple(out.shape)}")
+    _dequantize_rows(_device_of(q, scale, out), q.data_ptr(), ldq, scale.data_ptr(), n, width, out.data_ptr(), dtype_code(out), ldo)
     return out
 
 
@@ -686,31 +715,28 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
 
     ``x`` and ``residual``: bfloat16 or float32.  A row whose sum of squares or whose products with the weight
     leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row of zeros with ``eps = 0``."""
-    ld, code = _rows(x, "rmsnorm_q8"), dtype_code(x)
-    n, width = x.shape
-    if weight.dtype != torch.float32 or weight.dim() != 1 or not weight.is_contiguous() or weight.shape[0] != width:
+    n, width, ld = _dims(x, "rmsnorm_q8") if residual is None else _written_dims(x, "rmsnorm_q8")
+    code = dtype_code(x)
+    if weight.dtype is not torch.float32 or weight.shape != (width,) or not weight.is_contiguous():
         raise KernelError(f"rmsnorm_q8: the weight must be a contiguous float32 vector of {width}")
     if not eps >= 0:
         raise KernelError(f"rmsnorm_q8: eps must not be negative, got {eps}")
     if out is None:
         out = q8_rows(n, width, x.device)
-    if out.q.shape != x.shape:
-        raise KernelError(f"rmsnorm_q8: rows {tuple(x.shape)} do not go into {tuple(out.q.shape)}")
-    ldq = _written(_q8(out, "rmsnorm_q8"), out.q, "rmsnorm_q8")
-    ldr = rcode = r_ptr = 0
-    if residual is not None:
-        if residual.shape != x.shape:
-            raise KernelError(f"rmsnorm_q8: residual {tuple(residual.shape)} against x {tuple(x.shape)}")
-        ldr, rcode, r_ptr = _rows(residual, "rmsnorm_q8"), dtype_code(residual), residual.data_ptr()
-        _written(ld, x, "rmsnorm_q8")
-        dev = _device_of(x, weight, out.q, out.scale, residual)
+    q, scale = out
+    m, w, ldq = _q8_dims(out, "rmsnorm_q8", _written_dims)
+    if m != n or w != width:
+        raise KernelError(f"rmsnorm_q8: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
+    if residual is None:
+        r_ptr, r_code, ldr = None, 0, 0
+        dev = _device_of(x, weight, q, scale)
     else:
-        dev = _device_of(x, weight, out.q, out.scale)
-    f = _fn("quant", "skyla_rmsnorm_q8",
-            [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_float, c_void_p, c_int64,
-             c_void_p, c_void_p])
-    _launch_on(dev, "quant", f, x.data_ptr(), code, ld, r_ptr, rcode, ldr, n, width, weight.data_ptr(), eps,
-               out.q.data_ptr(), ldq, out.scale.data_ptr())
+        m, w, ldr = _dims(residual, "rmsnorm_q8")
+        if m != n or w != width:
+            raise KernelError(f"rmsnorm_q8: residual {tuple(residual.shape)} against x {tuple(x.shape)}")
+        r_ptr, r_code = residual.data_ptr(), dtype_code(residual)
+        dev = _device_of(x, weight, q, scale, residual)
+    _rmsnorm_q8(dev, x.data_ptr(), code, ld, r_ptr, r_code, ldr, n, width, weight.data_ptr(), eps, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
 
@@ -725,8 +751,7 @@ class Q8Weight:
     __slots__ = ("rows", "gated", "n_out", "n_in", "ld")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, gated: bool = False):
-        ld = _q8(Q8Rows(q, scale), "Q8Weight")
-        n, width = q.shape
+        n, width, ld = _q8_dims(Q8Rows(q, scale), "Q8Weight")
         if not 1 <= width <= Q8_MAX_WIDTH:
             raise KernelError(f"Q8Weight: {width} inputs are outside 1..{Q8_MAX_WIDTH}")
         if n < 1 or (gated and n % 2):
@@ -734,7 +759,7 @@ class Q8Weight:
         if ld % 16 or ld < width or q.data_ptr() % 16:
             kept = q8_rows(n, width, q.device).q
             kept.copy_(q)
-            q, ld = kept, _rows(kept, "Q8Weight")
+            q, ld = kept, _dims(kept, "Q8Weight")[2]
         if q.is_cuda:
             torch.cuda.current_stream(q.device).synchronize()
         self.rows, self.gated, self.n_in, self.ld = Q8Rows(q, scale), bool(gated), width, ld
@@ -763,35 +788,29 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
     ``mode``: STORE (``y = v``, bfloat16 or float32), ACCUMULATE (``y += v``, float32), GATED (``y = silu(gate) * up``
     of a gated weight, bfloat16).  ``x``'s rows should begin on multiples of 16 bytes (as :func:`q8_rows` makes
     them): others run on the plain kernel, with the same results."""
-    ldx = _q8(x, "linear_q8")
-    m, k = x.q.shape
+    q, scale = x
+    rows = w.rows
+    m, k, ldx = _q8_dims(x, "linear_q8")
     if k != w.n_in:
         raise KernelError(f"linear_q8: tokens of {k} against a weight of {w.n_in} inputs")
     if mode not in (STORE, ACCUMULATE, GATED) or (mode == GATED) != w.gated:
         raise KernelError(f"linear_q8: mode {mode} on a weight that is {'' if w.gated else 'not '}gated")
-    ldy, code = _rows(y, "linear_q8"), dtype_code(y)
-    if tuple(y.shape) != (m, w.n_out):
+    ym, yn, ldy = _written_dims(y, "linear_q8")
+    code = dtype_code(y)
+    if ym != m or yn != w.n_out:
         raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
-    if (mode == ACCUMULATE and code != F32) or (mode == GATED and code != BF16):
+    if code != (F32 if mode == ACCUMULATE else BF16 if mode == GATED else code):
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
-    _written(ldy, y, "linear_q8")
-    dev = _device_of(x.q, x.scale, w.rows.q, w.rows.scale, y)
+    dev = _device_of(q, scale, rows.q, rows.scale, y)
     if m == 1:
         ldx = w.ld  # the distance to a next row that is not there
-    if ldx % 16 == 0 and ldx >= k and x.q.data_ptr() % 16 == 0:
-        epilogue = {STORE: TC_STORE_F32 if code == F32 else TC_STORE_BF16, ACCUMULATE: TC_ACCUM_F32, GATED: TC_GLU_BF16}[mode]
-        f = _fn("gemm_q8", "skyla_linear_q8",
-                [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_int,
-                 c_void_p, c_void_p])
-        _launch_on(dev, "gemm_q8", f, x.q.data_ptr(), ldx, x.scale.data_ptr(), w.rows.q.data_ptr(), w.ld,
-                   w.rows.scale.data_ptr(), m, w.n_out, k, y.data_ptr(), ldy, epilogue,
-                   _state(state, y).error_flag.data_ptr())
-        return y
-    f = _fn("linear_q8_plain", "skyla_linear_q8_plain",
-            [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int64, c_int,
-             c_void_p])
-    _launch_on(dev, "linear_q8_plain", f, x.q.data_ptr(), ldx, x.scale.data_ptr(), w.rows.q.data_ptr(), w.ld,
-               w.rows.scale.data_ptr(), m, w.n_out, k, y.data_ptr(), code, ldy, mode)
+    if ldx % 16 == 0 and ldx >= k and q.data_ptr() % 16 == 0:
+        epilogue = TC_ACCUM_F32 if mode == ACCUMULATE else TC_GLU_BF16 if mode == GATED else TC_STORE_F32 if code == F32 else TC_STORE_BF16
+        _linear_q8(dev, q.data_ptr(), ldx, scale.data_ptr(), rows.q.data_ptr(), w.ld, rows.scale.data_ptr(), m, yn, k, y.data_ptr(), ldy,
+                   epilogue, _state(state, y).error_flag.data_ptr())
+    else:
+        _linear_q8_plain(dev, q.data_ptr(), ldx, scale.data_ptr(), rows.q.data_ptr(), w.ld, rows.scale.data_ptr(), m, yn, k, y.data_ptr(),
+                         code, ldy, mode)
     return y
 
 
