@@ -937,13 +937,10 @@ RowsPlan plan_rows(int N, int K, bool gated, int bn, bool fours) {
 }
 
 template <int BN, int MODE>
-int launch_rows(const Operands& o, const Args& a, cudaStream_t stream) {
+int launch_rows(const Operands& o, const Args& a, const RowsPlan& p, cudaStream_t stream) {
   constexpr bool gated = MODE == kGluBf16;
   constexpr int kATiles = gated ? 2 : 1;
   constexpr int M2 = gated ? kStoreBf16 : MODE;  // (no gated instance of the cluster and stacked kernels is built)
-  // the owners of a cluster write four neighbouring outputs of a token at once
-  const bool fours = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (MODE == kStoreBf16 ? 8 : 16) == 0;
-  const RowsPlan p = plan_rows(a.N, a.K, gated, BN, fours);
   CUtensorMap mw, mx;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, p.rows, p.kkb)) return rc;
   if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BN, p.kkb)) return rc;
@@ -992,22 +989,31 @@ int launch_rows(const Operands& o, const Args& a, cudaStream_t stream) {
   return check_launch("linear_q8");
 }
 
-// How a product of many tokens is cut: the accumulator's columns and the splits of K, whichever is done first by what
-// was measured (nanoseconds, 4,096 inputs at 130 to 2,048 tokens): a K block takes 370 / 245 / 205 at 256 / 128 / 64
-// columns, what a tile costs beside its K blocks is 5,200 / 3,450 / 2,800, a cluster's two meetings and the exchange
-// 3,500 (two blocks) or 4,700.  (A gated product of 200 tokens by the weight-streaming kernel, two instructions of 256
-// columns for 32 bytes of K: 39 against 30 us.)
-struct TilePlan { int columns, splits; };
+// What the two kernels were measured to take, in nanoseconds, for products of 17 to 2,048 tokens and the layer sizes
+// 4,096 / 6,144 / 12,288 / 25,600 and smaller odd ones (rules, right to about a tenth; none knows a size by name).
+// Weight streaming: a cluster's block takes 15 a KB of weight and tokens, and 70 for each token that it finishes; a block
+// with all of K 21 a KB (at least 300 a K block), and 60 a token for its short runs of outputs.
+double rows_ns(const RowsPlan& p, int M, int N, int K, bool gated, int bn, int sms) {
+  const int n_kb = (K + KB - 1) / KB;
+  if (p.splits > 1) {
+    const double kb = (n_kb + p.splits - 1) / p.splits;
+    return 3600 + 15.0 * kb * (p.rows + bn) * KB / 1024 + 70.0 * ((M + p.splits - 1) / p.splits);
+  }
+  const int waves = ((N + p.rows - 1) / p.rows + sms - 1) / sms;
+  const double stream = 21.0 * (p.rows * (gated ? 2 : 1) + bn) * KB / 1024;
+  return 3000 + (double)waves * n_kb * (stream > 300 ? stream : 300) + 60.0 * M;
+}
+// Tiles: a K block takes 370 / 245 / 205 at 256 / 128 / 64 columns, 540 / 300 / 205 where one tile of tokens reads each
+// weight once, from memory; a tile costs 5,200 / 3,450 / 2,800 beside its K blocks; a cluster's meetings and exchange
+// 2,900 (two blocks) or 4,200.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for
+// 32 bytes of K: 39 against 30 us.)
+struct TilePlan { int columns, splits; double ns; };
 TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
   const long long n_kb = (K + KB - 1) / KB, n_t = (M + BM - 1) / BM;
-  TilePlan best{256, 1};
-  double best_ns = 0;
-  auto offer = [&](int columns, int splits, double ns) {
-    if (best_ns == 0 || ns < best_ns) { best = TilePlan{columns, splits}; best_ns = ns; }
-  };
+  TilePlan best{256, 1, 0};
   for (int columns = 64; columns <= 256; columns *= 2) {
     if (gated && columns == 64) continue;
-    const double per_kb = columns == 256 ? 370 : columns == 128 ? 245 : 205;
+    const double per_kb = columns == 256 ? (n_t == 1 ? 540 : 370) : columns == 128 ? (n_t == 1 ? 300 : 245) : 205;
     const double beside = columns == 256 ? 5200 : columns == 128 ? 3450 : 2800;
     const int outputs = gated ? columns / 2 : columns;
     const long long tiles = n_t * ((N + outputs - 1) / outputs);
@@ -1016,7 +1022,8 @@ TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
       const long long waves = (tiles * splits + sms - 1) / sms;
       double main = (double)((n_kb + splits - 1) / splits) * per_kb;
       if (waves > 1 && main < beside / 2) main = beside / 2;  // (the epilogue of all but the last tile runs beside the next)
-      offer(columns, splits, (double)waves * main + beside + (splits == 2 ? 3500 : splits == 4 ? 4700 : 0));
+      const double ns = (double)waves * main + beside + (splits == 2 ? 2900 : splits == 4 ? 4200 : 0);
+      if (best.ns == 0 || ns < best.ns) best = TilePlan{columns, splits, ns};
     }
   }
   return best;
@@ -1082,13 +1089,21 @@ int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stre
 
 template <int MODE>
 int launch(const Operands& o, const Args& a, cudaStream_t stream) {
-  if (a.M <= 16) return launch_rows<16, MODE>(o, a, stream);
-  if (a.M <= 32) return launch_rows<32, MODE>(o, a, stream);
-  if (a.M <= 64) return launch_rows<64, MODE>(o, a, stream);
-  if (a.M <= 128) return launch_rows<128, MODE>(o, a, stream);
-  const TilePlan p = plan_tiles(a.M, a.N, a.K, MODE == kGluBf16, sm_count());
+  constexpr bool gated = MODE == kGluBf16;
+  const int bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+  const int sms = sm_count();
+  // the owners of a cluster write four neighbouring outputs of a token at once
+  const bool fours = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (MODE == kStoreBf16 ? 8 : 16) == 0;
+  const RowsPlan r = plan_rows(a.N, a.K, gated, bn, fours);
+  if (a.M <= 16) return launch_rows<16, MODE>(o, a, r, stream);
+  const TilePlan p = plan_tiles(a.M, a.N, a.K, gated, sms);
+  if (a.M <= 128 && rows_ns(r, a.M, a.N, a.K, gated, bn, sms) < p.ns) {
+    if (bn == 32) return launch_rows<32, MODE>(o, a, r, stream);
+    if (bn == 64) return launch_rows<64, MODE>(o, a, r, stream);
+    return launch_rows<128, MODE>(o, a, r, stream);
+  }
   if (p.columns == 256) return launch_tiles<MODE, 256>(o, a, p.splits, stream);
-  if (p.columns == 64 && MODE != kGluBf16) return launch_tiles<MODE == kGluBf16 ? kStoreBf16 : MODE, 64>(o, a, p.splits, stream);
+  if (p.columns == 64) return launch_tiles<gated ? kStoreBf16 : MODE, 64>(o, a, p.splits, stream);  // (no gated tile is this narrow)
   return launch_tiles<MODE, 128>(o, a, p.splits, stream);
 }
 }  // namespace
