@@ -456,6 +456,8 @@ __device__ __forceinline__ void put16(uint32_t row_smem, int row, int c, uint32_
 struct TileArgs {
   int by_tma;         // map_y is y's: outputs leave by TMA
   int boxes;          // the maps of x and w bring a stage's K blocks at once (K in whole blocks); else one by one
+  int x_rows;         // rows of a box of x: 128, or the tokens of a single tile to the next eight (the MMA then reads what
+                      // lies behind them as rows that nobody reads).  Boxes that reach far beyond the tokens are slow.
   int n_t_tiles, n_tiles;
   int splits;         // blocks of a cluster (SPLIT), each with an equal run of the K blocks; else 1
 };
@@ -513,6 +515,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
   constexpr int kKkb = C::kKkb;
   const int n_st = (kb_hi - kb_lo + kKkb - 1) / kKkb;  // stages of a tile
+  const int x_bytes = ta.x_rows * KB;                  // of a K block: a multiple of 1024
 
   if (warp == 0) {
     if (lane == 0) {
@@ -526,7 +529,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         auto load_weights = [&](int i, int s) {
           const int kb = kb_lo + i * kKkb;
           const uint32_t sw = base + s * C::kStageBytes + kKkb * C::kXBytes;
-          mbar_expect_tx(full_bar(s), C::kStageBytes);
+          mbar_expect_tx(full_bar(s), (uint32_t)(kKkb * (x_bytes + C::kWBytes)));
           if (MODE == kGluBf16) {
             tma_load_2d(sw, &map_w, full_bar(s), kb * KB, row0);
             tma_load_2d(sw + C::kWBytes / 2, &map_w, full_bar(s), kb * KB, a.N + row0);
@@ -556,7 +559,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             tma_load_3d(sx, &map_x, full_bar(s), 0, t_tile * BM, kb);
           } else {
 #pragma unroll
-            for (int j = 0; j < kKkb; ++j) tma_load_2d(sx + j * C::kXBytes, &map_x, full_bar(s), (kb + j) * KB, t_tile * BM);
+            for (int j = 0; j < kKkb; ++j) tma_load_2d(sx + j * x_bytes, &map_x, full_bar(s), (kb + j) * KB, t_tile * BM);
           }
           armed |= 1u << s;
           armed_parity = (armed_parity & ~(1u << s)) | (phase << s);
@@ -590,7 +593,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
           for (int j = 0; j < kKkb; ++j) {
             if (kb_lo + i * kKkb + j >= kb_hi) break;
-            const uint64_t dx = umma_desc(sx + j * C::kXBytes), dw = umma_desc(sw + j * C::kWBytes);
+            const uint64_t dx = umma_desc(sx + j * x_bytes), dw = umma_desc(sw + j * C::kWBytes);
 #pragma unroll
             for (int k = 0; k < KB / 32; ++k) {
               umma_i8(d, dx + 2 * k, dw + 2 * k, idesc, started);
@@ -1042,7 +1045,8 @@ int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stre
   CUtensorMap mx, mw, my;
   ta.boxes = C::kKkb > 1 && a.K % KB == 0;
   const int kkb = ta.boxes ? C::kKkb : 1;
-  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, kkb)) return rc;
+  ta.x_rows = a.M < BM ? (a.M + 7) / 8 * 8 : BM;
+  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, ta.x_rows, kkb)) return rc;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, MODE == kGluBf16 ? BF / 2 : BF, kkb)) return rc;
   const int size = f32 ? 4 : 2;
   // (a TMA store clips at whole 16-byte pieces: a row that ends inside one would write beyond it)
