@@ -134,13 +134,14 @@ class _Tokens:
 
 def load(model: Union[str, dict, object], dtype: str = "bfloat16", max_tokens: int = 4096,
          max_slots: Optional[int] = None, device="cuda:0", seed: int = 0,
-         linear_std: float = 0.02, norm_std: float = 0.02) -> Model:
+         linear_std: float = 0.02, norm_std: float = 0.02, weights: Optional[str] = None) -> Model:
     """``model``: a folder with config.json and model.safetensors, or a configuration
     (a dict in config.json form or a configuration object) to fill with seeded
-    random weights."""
+    random weights.  ``weights="int8"`` (with ``dtype="bfloat16"``): the layers' matrices are
+    quantised to 8-bit integers as they are loaded, and their products run on them."""
     if isinstance(model, (str, os.PathLike)):
-        return Model(Engine.from_folder(os.fspath(model), dtype, max_tokens, max_slots, device))
+        return Model(Engine.from_folder(os.fspath(model), dtype, max_tokens, max_slots, device, weights=weights))
     config = config_from_dict(model) if isinstance(model, dict) else model
     store = torch.float32 if dtype in ("float32", "fp32") else torch.bfloat16
     tensors = random_tensors(declared_tensors(config.to_spec()), seed, store, linear_std, norm_std)
-    return Model(Engine(config, tensors, dtype, max_tokens, max_slots, device))
+    return Model(Engine(config, tensors, dtype, max_tokens, max_slots, device, weights=weights))

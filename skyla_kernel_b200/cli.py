@@ -4,11 +4,11 @@ docs/roadmap.md:186,230-231) plus what a library without a tokenizer needs: toke
 a random-weights writer and the replay program.
 
     skyla run MODEL --prompt-ids 1,2,3 -n 16 [--temperature T --top-k K --top-p P --seed S]
-                    [--dtype bfloat16|float32] [--check] [--profile] [--warmup]
-    skyla bench MODEL [--batch 8] [--prompt-len 512] [-n 64]
+                    [--dtype bfloat16|float32] [--weights int8] [--check] [--profile] [--warmup]
+    skyla bench MODEL [--batch 8] [--prompt-len 512] [-n 64] [--weights int8]
     skyla bench-bw [--mib 512] [--reps 9]
     skyla random --config CONFIG.json --out DIR [--seed S] [--dtype bfloat16|float32]
-    skyla kernel-bench linear|attention-decode|attention-prefill|step [sizes]
+    skyla kernel-bench linear|linear-int8|norm-int8|quantize|attention-decode|attention-prefill|step [sizes]
     skyla replay --model DIR --dtype D --out DIR --max-tokens N   (same as bin/trace_run)
 """
 from __future__ import annotations
@@ -31,7 +31,7 @@ def cmd_run(a) -> int:
     from .engine import StepItem
     prompts = [_ids(p) for p in a.prompt_ids]
     pages = sum(-(-(len(p) + a.n) // 64) for p in prompts)
-    model = load(a.model, dtype=a.dtype, max_tokens=max(a.max_tokens or 0, 64 * pages))
+    model = load(a.model, dtype=a.dtype, max_tokens=max(a.max_tokens or 0, 64 * pages), weights=a.weights)
     kw = dict(max_new_tokens=a.n, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, seed=a.seed,
               stop_ids=a.stop_id if a.stop_id is not None else None)
     if a.warmup:  # as the reference: the prompt once first (README.md:247)
@@ -97,8 +97,8 @@ def _check(a, prompts, out) -> int:
     from . import load
     from .engine import StepItem
     worst_all, mismatches, real = 0.0, 0, 0
-    engines = [load(a.model, dtype=d, max_tokens=64 * (-(-(max(map(len, prompts)) + a.n) // 64))).engine
-               for d in (a.dtype, "float32")]
+    engines = [load(a.model, dtype=d, max_tokens=64 * (-(-(max(map(len, prompts)) + a.n) // 64)), weights=w).engine
+               for d, w in ((a.dtype, a.weights), ("float32", None))]
     for p, o in zip(prompts, out):
         slots = [e.alloc_slot() for e in engines]
         feed = list(p)
@@ -127,7 +127,7 @@ def cmd_bench(a) -> int:
     from . import load
     from .engine import StepItem
     max_tokens = a.batch * 64 * (-(-(a.prompt_len + a.n + 8) // 64))
-    model = load(a.model, dtype=a.dtype, max_tokens=max_tokens)
+    model = load(a.model, dtype=a.dtype, max_tokens=max_tokens, weights=a.weights)
     eng = model.engine
     g = torch.Generator().manual_seed(0)
     prompts = [torch.randint(0, eng.vocab_size, (a.prompt_len,), generator=g).tolist() for _ in range(a.batch)]
@@ -204,6 +204,7 @@ def main(argv=None) -> int:
         p.add_argument("--seed", type=int, default=0)
         p.add_argument("--stop-id", type=int, action="append")
         p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+        p.add_argument("--weights", choices=["int8"], help="the layers' products on 8-bit integers (with bfloat16)")
         p.add_argument("--max-tokens", type=int, default=0)
         p.add_argument("--check", action="store_true", help="lockstep against the 32-bit path")
         p.add_argument("--profile", action="store_true", help="per-stage times of one decode step")
@@ -215,6 +216,7 @@ def main(argv=None) -> int:
     p.add_argument("--prompt-len", type=int, default=512)
     p.add_argument("-n", type=int, default=64)
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--weights", choices=["int8"], help="the layers' products on 8-bit integers (with bfloat16)")
     p.set_defaults(fn=cmd_bench)
     p = sub.add_parser("bench-bw", help="streaming-read bandwidth of the device")
     p.add_argument("--mib", type=int, default=512)
@@ -229,7 +231,7 @@ def main(argv=None) -> int:
     p.add_argument("--norm-std", type=float, default=0.02)
     p.set_defaults(fn=cmd_random)
     p = sub.add_parser("kernel-bench", help="time one kernel on its own (also the target of profiler captures)")
-    p.add_argument("kernel", choices=["linear", "attention-decode", "attention-prefill", "step"])
+    p.add_argument("kernel", choices=["linear", "linear-int8", "norm-int8", "quantize", "attention-decode", "attention-prefill", "step"])
     p.add_argument("--layers", type=int, default=4, help="step: layers of the 8B-shaped model")
     p.add_argument("--tokens", type=int, default=8)
     p.add_argument("--n-out", type=int, default=4096)
@@ -239,6 +241,7 @@ def main(argv=None) -> int:
     p.add_argument("--batch", type=int, default=8)
     p.add_argument("--context", type=int, default=2048)
     p.add_argument("--reps", type=int, default=5)
+    p.add_argument("--weights", choices=["int8"], help="the layers' products on 8-bit integers (step)")
     p.set_defaults(fn=lambda a: __import__("skyla_kernel_b200.kernel_bench", fromlist=["main"]).main(a))
     p = sub.add_parser("replay", help="replay a token trace from standard input (bin/trace_run)")
     p.add_argument("--model", required=True)

@@ -46,14 +46,16 @@ class Engine:
     (default: one per page).  ``tensors`` (checkpoint name -> tensor) is consumed:
     parts take out of it what they copy into matrices of their own, so that a
     caller who keeps no other reference keeps no second copy of the weights.
+    ``weights="int8"`` (with ``dtype="bfloat16"``) quantises the layers' matrices when they are loaded
+    and runs their products on 8-bit integers (``parts.linear.Q8Linear``).
     """
 
     def __init__(self, config, tensors: Dict[str, torch.Tensor], dtype: str = "bfloat16",
                  max_tokens: int = 4096, max_slots: Optional[int] = None, device="cuda:0",
-                 cuda_graphs: Optional[bool] = None):
+                 cuda_graphs: Optional[bool] = None, weights: Optional[str] = None):
         self.config = config
         self.spec = config.to_spec()
-        self.rt = Runtime(_device(device), dtype)
+        self.rt = Runtime(_device(device), dtype, weights=weights)
         torch.cuda.set_device(self.rt.device)
         self.model = DecoderModel(self.spec, self.rt)
         kernel_build.build_all(self.model.kernels_needed())
@@ -71,11 +73,12 @@ class Engine:
     # ---------------------------------------------------------------- loading
     @classmethod
     def from_folder(cls, folder: str, dtype: str = "bfloat16", max_tokens: int = 4096,
-                    max_slots: Optional[int] = None, device="cuda:0", cuda_graphs: Optional[bool] = None) -> "Engine":
+                    max_slots: Optional[int] = None, device="cuda:0", cuda_graphs: Optional[bool] = None,
+                    weights: Optional[str] = None) -> "Engine":
         config = config_from_folder(folder)
         spec = config.to_spec()
         tensors = load_weights(folder, declared_tensors(spec), spec.optional_tensors)
-        return cls(config, tensors, dtype, max_tokens, max_slots, device, cuda_graphs)
+        return cls(config, tensors, dtype, max_tokens, max_slots, device, cuda_graphs, weights)
 
     # ------------------------------------------------------------------ slots
     def alloc_slot(self) -> int:

@@ -3,6 +3,8 @@ different weights so that nothing is served from L2), the way the reference time
 dispatch (skyla-vk/src/submit.rs:31-76).  Also the target of profiler captures:
 
     skyla kernel-bench linear --tokens 8 --n-out 4096 --n-in 12288 --mode accumulate
+    skyla kernel-bench linear-int8 --tokens 8 --n-out 4096 --n-in 12288 --mode accumulate
+    skyla kernel-bench norm-int8|quantize --tokens 2048 --n-in 4096
     skyla kernel-bench attention-decode --batch 8 --context 2048
     skyla kernel-bench attention-prefill --tokens 2048
     skyla kernel-bench step --tokens 2048 --batch 1 --layers 4      (a prompt step of the 8B layer sizes)
@@ -94,6 +96,41 @@ def linear(tokens: int, n_out: int, n_in: int, mode: str, copies: int = 0, reps:
             "rows_kernel": lins[0].streams(tokens), "plan": lins[0].rows_plans[ops.token_tile(min(tokens, ops.ROWS_MAX_TOKENS))]}
 
 
+def linear_int8(tokens: int, n_out: int, n_in: int, mode: str, copies: int = 0, reps: int = 5) -> dict:
+    """The product in 8-bit integers (tokens already quantised)."""
+    if mode not in ("store", "store-f32", "accumulate", "gated"):
+        raise ValueError(f"linear-int8 has no mode {mode}")
+    gated = mode == "gated"
+    rows = n_out * (2 if gated else 1)
+    copies = copies or max(2, min(24, int(400e6 // (rows * n_in)) + 1))  # > L2 in total
+    weights = []
+    for i in range(copies):
+        w = torch.empty(rows, n_in, dtype=torch.bfloat16, device=DEV)
+        ops.fill_normal(w, 0.0, 0.02, i)
+        weights.append(ops.Q8Weight.quantize(w, gated))
+    x = ops.quantize_rows(torch.randn(tokens, n_in, device=DEV))
+    y = torch.zeros(tokens, n_out, device=DEV, dtype=torch.float32 if mode in ("accumulate", "store-f32") else torch.bfloat16)
+    how = ops.GATED if gated else ops.ACCUMULATE if mode == "accumulate" else ops.STORE
+    us = _time(lambda i: ops.linear_q8(x, weights[i], y, how), copies, reps)
+    return {"kernel": "linear-int8", "tokens": tokens, "n_out": n_out, "n_in": n_in, "mode": mode, "us": us,
+            "weight_GBps": rows * n_in / us / 1e3, "TOPs": 2.0 * tokens * rows * n_in / us / 1e6}
+
+
+def rows_int8(kernel: str, tokens: int, width: int, reps: int = 5) -> dict:
+    """The norm (32-bit rows, a bfloat16 residual added) or the quantisation (bfloat16 rows) that leaves 8-bit rows."""
+    copies = max(2, min(24, int(400e6 // (tokens * width * 4)) + 1))
+    out = [ops.q8_rows(tokens, width, DEV) for _ in range(copies)]
+    if kernel == "quantize":
+        x = [torch.randn(tokens, width, device=DEV).to(torch.bfloat16) for _ in range(copies)]
+        us, moved = _time(lambda i: ops.quantize_rows(x[i], out[i]), copies, reps), 3
+    else:
+        x = [torch.randn(tokens, width, device=DEV) for _ in range(copies)]
+        r = [torch.randn(tokens, width, device=DEV).to(torch.bfloat16) for _ in range(copies)]
+        w = torch.ones(width, device=DEV)
+        us, moved = _time(lambda i: ops.rmsnorm_q8(x[i], w, 1e-6, out[i], r[i]), copies, reps), 11
+    return {"kernel": kernel, "tokens": tokens, "width": width, "us": us, "GBps": moved * tokens * width / us / 1e3}
+
+
 def _paged(batch: int, context: int, nkv: int, hd: int):
     pages = -(-context // 64)
     width = 8
@@ -142,7 +179,7 @@ def attention_prefill(tokens: int, nq: int = 32, nkv: int = 8, hd: int = 128, re
     return {"kernel": "attention-prefill", "tokens": tokens, "us": us, "TFLOPs": flops / us / 1e6}
 
 
-def step(tokens: int, batch: int, context: int, layers: int, reps: int = 3) -> dict:
+def step(tokens: int, batch: int, context: int, layers: int, reps: int = 3, weights=None) -> dict:
     """Whole steps of a model with the Qwen3-8B layer sizes and ``layers`` layers, random weights drawn on
     the device: ``batch`` prompts of ``tokens`` tokens in one step (``tokens`` > 1), or one token for each
     of ``batch`` sequences that hold ``context`` positions (``tokens`` == 1).  With an event after each
@@ -152,7 +189,7 @@ def step(tokens: int, batch: int, context: int, layers: int, reps: int = 3) -> d
     from .engine import StepItem
     from .measure import random_engine
     length = tokens if tokens > 1 else context
-    eng, cfg = random_engine("8b", layers, max_tokens=batch * (length + 128), max_slots=batch, device=DEV)
+    eng, cfg = random_engine("8b", layers, max_tokens=batch * (length + 128), max_slots=batch, device=DEV, weights=weights)
     g = torch.Generator().manual_seed(1)
     prompts = [torch.randint(0, cfg.vocab_size, (length,), generator=g).tolist() for _ in range(batch)]
     times = []
@@ -183,16 +220,20 @@ def step(tokens: int, batch: int, context: int, layers: int, reps: int = 3) -> d
     for label, ns in eng.last_step_profile():
         stages[label] = stages.get(label, 0.0) + ns / 1e3
     timed = sorted(times[-1 - reps:-1])
-    return {"kernel": "step", "tokens": tokens, "batch": batch, "context": length, "layers": layers,
+    return {"kernel": "step", "tokens": tokens, "batch": batch, "context": length, "layers": layers, "weights": weights or "bfloat16",
             "ms": timed[len(timed) // 2], "ms_with_stage_events": times[-1],
             "stage_us": {k: round(v, 1) for k, v in stages.items()}}
 
 
 def main(a) -> int:
     if a.kernel == "step":
-        r = step(a.tokens, a.batch, a.context, a.layers, reps=a.reps)
+        r = step(a.tokens, a.batch, a.context, a.layers, reps=a.reps, weights=a.weights)
     elif a.kernel == "linear":
         r = linear(a.tokens, a.n_out, a.n_in, a.mode, reps=a.reps)
+    elif a.kernel == "linear-int8":
+        r = linear_int8(a.tokens, a.n_out, a.n_in, a.mode, reps=a.reps)
+    elif a.kernel in ("norm-int8", "quantize"):
+        r = rows_int8(a.kernel, a.tokens, a.n_in, reps=a.reps)
     elif a.kernel == "attention-decode":
         r = attention_decode(a.batch, a.context, reps=a.reps)
     else:

@@ -46,14 +46,15 @@ def random_tensors_on_device(cfg, seed: int = 0, store: torch.dtype = torch.bflo
 
 def random_engine(shape: Union[str, dict], layers: Optional[int] = None, max_tokens: int = 4096,
                   max_slots: Optional[int] = None, seed: int = 0, dtype: str = "bfloat16", device="cuda:0",
-                  linear_std: float = 0.02, norm_std: float = 0.02):
+                  linear_std: float = 0.02, norm_std: float = 0.02, weights: Optional[str] = None):
     """(engine, configuration) of a model with the layer sizes of ``shape`` (a key of ``SHAPES`` or a
-    config.json-style dict) and ``layers`` layers (default: the shape's own), with random weights."""
+    config.json-style dict) and ``layers`` layers (default: the shape's own), with random weights
+    (``weights="int8"``: the layers' products on 8-bit integers)."""
     from .engine import Engine
     cfg = random_config(shape, layers)
     store = torch.float32 if dtype in ("float32", "fp32") else torch.bfloat16
     tensors = random_tensors_on_device(cfg, seed, store, device, linear_std, norm_std)
-    engine = Engine(cfg, tensors, dtype, max_tokens=max_tokens, max_slots=max_slots, device=device)
+    engine = Engine(cfg, tensors, dtype, max_tokens=max_tokens, max_slots=max_slots, device=device, weights=weights)
     del tensors
     torch.cuda.empty_cache()
     return engine, cfg

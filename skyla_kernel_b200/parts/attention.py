@@ -29,7 +29,7 @@ from ..cache.kv import KVNeed
 from ..kernels import ops
 from ..weights.loader import TensorDecl
 from .base import NormedInput, Part, StepPlan, build_part, register_mixer
-from .linear import ACCUMULATE, STORE, Linear
+from .linear import ACCUMULATE, STORE, Linear, layer_kernels, layer_linear
 
 
 class DecodePages(StepPlan):
@@ -135,9 +135,9 @@ class GQAttention(Part):
             parts = [w.to(torch.float32) for w in parts]
         fused = self.rt.matrix(torch.cat(parts, dim=0))
         del parts
-        self.qkv = Linear(fused, self.rt)
-        self.q_only = Linear(fused[: self.nq * self.hd], self.rt)
-        self.out = Linear(self.rt.matrix(tensors[t["o_proj"]]), self.rt)
+        self.qkv = layer_linear(fused, self.rt)
+        self.q_only = self.qkv.first_outputs(self.nq * self.hd)
+        self.out = layer_linear(self.rt.matrix(tensors[t["o_proj"]]), self.rt)
         if self.qk_norm:
             self.q_norm_w = self.rt.vector(tensors[t["q_norm"]])
             self.k_norm_w = self.rt.vector(tensors[t["k_norm"]])
@@ -146,7 +146,7 @@ class GQAttention(Part):
         return self.qkv.bytes() + self.out.bytes()
 
     def kernels_needed(self):
-        return self.kernel_modules
+        return tuple(dict.fromkeys(self.kernel_modules + layer_kernels(self.rt)))
 
     # -------------------------------------------------------------------- cache
     def _decode_plan(self, ctx, pages):
@@ -176,7 +176,9 @@ class GQAttention(Part):
         few = entry.owns_cache and self.qkv.streams(n) and self.rt.act_dtype == torch.bfloat16
         scale_in = None
         if isinstance(h, NormedInput):
-            if ((few or (entry.owns_cache and self.qkv.prompts(n))) and h.ahead is not None
+            if self.qkv.takes_rows:
+                h = h.rows()
+            elif ((few or (entry.owns_cache and self.qkv.prompts(n))) and h.ahead is not None
                     and ops.tc_linear_ok(h.ahead[0], self.qkv.weight)):
                 scale_in = (h.ahead[1], h.norm.rms_scale_form()[1])  # the product that wrote x last left x * norm weight
                 h = h.ahead[0]

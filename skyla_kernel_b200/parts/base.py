@@ -14,7 +14,8 @@ Interfaces (``ctx`` is the step's :class:`~skyla_kernel_b200.engine.batch.StepCo
 * norm           ``forward(ctx, x, out, rows=None)``: ``out[r] = norm(x[rows[r]])``; a norm of
                  the form "one scalar per row times a fixed vector" may say so with
                  ``rms_scale_form()`` (see ``parts/norm.py``), which lets the product before
-                 it prepare its input
+                 it prepare its input; one that can leave its rows in 8 bits has
+                 ``forward_rows(ctx, x, out)``
 * mixer          ``cache_need()``, ``state_need()``, ``forward(ctx, h, x, entry)``:
                  adds its output to ``x``; ``entry`` says which cache it uses
 * feed-forward   ``forward(ctx, h, x)``: adds its output to ``x``
@@ -41,6 +42,9 @@ class Runtime:
     ``float32``: weights, cache and activations in 32-bit, plain kernels only.
     ``bfloat16``: 16-bit weights, cache and matrix-product operands; the residual
     stream, norms, softmax, rotation and accumulation stay 32-bit.
+    ``weights="int8"`` (with ``bfloat16``): the layers' matrix products take weights and
+    tokens in 8-bit integers, a scale for every output and every token; embedding and
+    head, cache and attention stay 16-bit.
     """
 
     device: torch.device
@@ -51,6 +55,8 @@ class Runtime:
     #: {blocks per cluster: clusters of the weight-streaming kernel that run at a time}; asked from the device
     #: when not given
     cluster_room: Optional[dict] = None
+    #: ``None`` (in the runtime's precision) or ``"int8"``
+    weights: Optional[str] = None
 
     def __post_init__(self):
         if self.dtype in ("fp32", "float"):
@@ -59,6 +65,10 @@ class Runtime:
             self.dtype = "bfloat16"
         if self.dtype not in ("float32", "bfloat16"):
             raise ValueError(f"dtype must be float32 or bfloat16, not {self.dtype!r}")
+        if self.weights not in (None, "int8"):
+            raise ValueError(f"weights must be None or int8, not {self.weights!r}")
+        if self.weights == "int8" and self.dtype != "bfloat16":
+            raise ValueError("weights in int8 go with dtype bfloat16")
         self.device = torch.device(self.device)
         self._placed = {}
         self.shared_parts = {}
@@ -126,6 +136,11 @@ class Runtime:
             self._placed[id(t)] = (t, placed)
         return placed
 
+    @property
+    def int8(self) -> bool:
+        """Whether the layers' products run on 8-bit integers."""
+        return self.weights == "int8"
+
     def vector(self, t: torch.Tensor) -> torch.Tensor:
         """A norm weight or other small table: always 32-bit on the device."""
         return t.to(device=self.device, dtype=torch.float32).contiguous()
@@ -185,18 +200,26 @@ class StepPlan:
         positions and bring ``ns[b]`` new tokens."""
 
 
+def q8_buffer(ctx, name: str, n: int, width: int):
+    """Room in the step's workspace for ``n`` rows of ``width`` in 8 bits, each on a multiple of 16 bytes."""
+    from ..kernels.ops import Q8Rows
+    q = ctx.buffer(name + ".q8", (n, -(-width // 16) * 16), torch.int8)
+    return Q8Rows(q[:, :width], ctx.buffer(name + ".q8_scale", (n,), torch.float32))
+
+
 class NormedInput:
     """The input of a mixer or feed-forward before it is computed: ``norm(x)``.
 
     A block hands this to parts that set ``takes_normed_input = True``; such a part either
-    calls :meth:`tensor` (the norm runs as a kernel of its own) or, where the product that
-    wrote ``x`` last prepared the norm's input (:attr:`ahead`), feeds that to its first product.
+    calls :meth:`tensor` (the norm runs as a kernel of its own), or :meth:`rows` for a product
+    in 8 bits, or, where the product that wrote ``x`` last prepared the norm's input
+    (:attr:`ahead`), feeds that to its first product.
     Parts without the flag get ``tensor()``.
     """
 
     def __init__(self, ctx, x: torch.Tensor, norm):
         self.ctx, self.x, self.norm = ctx, x, norm
-        self._tensor = None
+        self._tensor = self._rows = None
         #: (x * norm.weight in bfloat16, shares of the rows' sums of squares) where the product that
         #: wrote ``x`` last left them (``Linear.forward(..., ctx=ctx)``); a part may feed them to its
         #: first product (``scale_in=``) instead of calling :meth:`tensor`
@@ -210,6 +233,23 @@ class NormedInput:
             ctx.mark("rmsnorm")
             self._tensor = h
         return self._tensor
+
+    def rows(self):
+        """The normed rows in 8 bits (``ops.Q8Rows``): left by the norm itself if it can
+        (``norm.forward_rows``), else made from :meth:`tensor`."""
+        if self._rows is None:
+            ctx, x = self.ctx, self.x
+            out = q8_buffer(ctx, "block.normed", ctx.n_tokens, x.shape[1])
+            if hasattr(self.norm, "forward_rows"):
+                self.norm.forward_rows(ctx, x, out)
+                ctx.mark("rmsnorm, 8 bits")
+            else:
+                h = self.tensor()
+                from ..kernels import ops
+                ops.quantize_rows(h, out)
+                ctx.mark("quantize")
+            self._rows = out
+        return self._rows
 
 
 _REGISTRIES: Dict[str, Dict[str, type]] = {

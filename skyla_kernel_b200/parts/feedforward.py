@@ -15,7 +15,7 @@ import torch
 from ..weights.loader import TensorDecl
 from ..kernels import ops
 from .base import NormedInput, Part, register_feed_forward
-from .linear import ACCUMULATE, GATED, Linear
+from .linear import ACCUMULATE, GATED, Linear, layer_kernels, layer_linear
 
 
 def fuse_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -49,8 +49,11 @@ class SwiGLU(Part):
             gate, up = gate.to(torch.float32), up.to(torch.float32)
         fused = fuse_gate_up(gate, up)
         del gate, up
-        self.gate_up = Linear(self.rt.matrix(fused), self.rt, gated=True)
-        self.down = Linear(self.rt.matrix(tensors[t["down_proj"]]), self.rt)
+        self.gate_up = layer_linear(self.rt.matrix(fused), self.rt, gated=True)
+        self.down = layer_linear(self.rt.matrix(tensors[t["down_proj"]]), self.rt)
+
+    def kernels_needed(self):
+        return tuple(dict.fromkeys(self.kernel_modules + layer_kernels(self.rt)))
 
     def weight_bytes(self) -> int:
         return self.gate_up.bytes() + self.down.bytes()
@@ -59,7 +62,9 @@ class SwiGLU(Part):
         act = ctx.buffer("ffn.act", (ctx.n_tokens, self.inter), self.rt.act_dtype)
         scale_in = None
         if isinstance(h, NormedInput):
-            if (h.ahead is not None and self.gate_up.takes_scale_in(ctx.n_tokens)
+            if self.gate_up.takes_rows:
+                h = h.rows()
+            elif (h.ahead is not None and self.gate_up.takes_scale_in(ctx.n_tokens)
                     and ops.tc_linear_ok(h.ahead[0], self.gate_up.weight)):
                 scale_in = (h.ahead[1], h.norm.rms_scale_form()[1])  # the product that wrote x last left x * norm weight
                 h = h.ahead[0]

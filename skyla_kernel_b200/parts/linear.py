@@ -3,18 +3,22 @@
 ``y = x W^T`` with ``W`` stored ``[outputs, inputs]`` (skyla-ref/src/matrix.rs:38-58).
 The plain 32-bit kernel takes every shape and dtype; the tensor-core and
 bandwidth-bound bfloat16 kernels take the shapes they are written for and are
-chosen here, never by the caller.
+chosen here, never by the caller.  :func:`layer_linear` gives the layers their products:
+in the runtime's precision, or in 8-bit integers where the runtime says so.
 """
 from __future__ import annotations
 
 import torch
 
 from ..kernels import ops
+from .base import q8_buffer
 
 STORE, ACCUMULATE, GATED = ops.STORE, ops.ACCUMULATE, ops.GATED
 
 
 class Linear:
+    #: whether :meth:`forward` takes 8-bit rows (``NormedInput.rows``)
+    takes_rows = False
     kernel_modules = ("linear_plain", "gemm_tc", "gemm_prompt")
 
     #: inputs from which a product of 65 to 128 tokens that the weight-streaming kernel does not take goes to
@@ -145,3 +149,61 @@ class Linear:
 
     def bytes(self) -> int:
         return self.weight.numel() * self.weight.element_size()
+
+    def first_outputs(self, n: int) -> "Linear":
+        """The product with the weight's first ``n`` outputs only, on the same memory."""
+        return Linear(self.weight[:n], self.rt)
+
+
+class Q8Linear:
+    """A layer's product in 8-bit integers (``ops.linear_q8``, which picks the kernel): the weight is quantised when
+    it is loaded, a scale for every output, and the tokens on the way in, a scale for each."""
+
+    takes_rows = True
+    kernel_modules = ("gemm_q8", "linear_q8_plain", "quant")
+    #: steps of up to this many tokens leave whole 32-bit rows of q, k and v for the kernels that finish them
+    ROWS_MAX_TOKENS = Linear.ROWS_MAX_TOKENS
+    #: and decode steps of up to this many have them finished inside the attention kernel
+    STACKED_MAX_TOKENS = Linear.STACKED_MAX_TOKENS
+
+    def __init__(self, weight, rt, gated: bool = False):
+        """``weight`` on the device, or an ``ops.Q8Weight``."""
+        self.weight = weight if isinstance(weight, ops.Q8Weight) else ops.Q8Weight.quantize(weight, gated)
+        self.rt = rt
+        self.gated, self.n_in, self.n_out = self.weight.gated, self.weight.n_in, self.weight.n_out
+
+    def streams(self, m: int) -> bool:
+        return m <= self.ROWS_MAX_TOKENS
+
+    def prompts(self, m: int) -> bool:
+        """No kernel of this product finishes the q, k and v heads in its epilogue."""
+        return False
+
+    def takes_scale_in(self, m: int) -> bool:
+        return False
+
+    def forward(self, x, y: torch.Tensor, mode: int = STORE, scale_in=None, ctx=None) -> torch.Tensor:
+        """``x``: 8-bit rows, or tokens to be quantised (in the workspace of ``ctx``, if there is one)."""
+        if scale_in is not None:
+            raise ValueError("a product in 8 bits takes no scale_in (takes_scale_in)")
+        if ctx is not None:
+            ctx.next_norm = None  # nothing is prepared for the norm that reads y next
+        if not isinstance(x, ops.Q8Rows):
+            x = ops.quantize_rows(x, q8_buffer(ctx, "linear", *x.shape) if ctx is not None else None)
+        return ops.linear_q8(x, self.weight, y, GATED if self.gated else mode, state=self.rt.kernel_state)
+
+    def first_outputs(self, n: int) -> "Q8Linear":
+        return Q8Linear(self.weight.first_outputs(n), self.rt)
+
+    def bytes(self) -> int:
+        return self.weight.bytes()
+
+
+def layer_linear(weight: torch.Tensor, rt, gated: bool = False):
+    """The product of a layer's weight (on the device) in the form that the runtime asks for."""
+    return Q8Linear(weight, rt, gated) if rt.int8 else Linear(weight, rt, gated)
+
+
+def layer_kernels(rt):
+    """The kernel libraries of :func:`layer_linear`'s products."""
+    return Q8Linear.kernel_modules if rt.int8 else Linear.kernel_modules

@@ -34,6 +34,13 @@ class RMSNorm(Part):
     def forward(self, ctx, x: torch.Tensor, out: torch.Tensor, rows: Optional[torch.Tensor] = None):
         return ops.rmsnorm(x, self.weight, self.eps, out, rows)
 
+    def forward_rows(self, ctx, x: torch.Tensor, out: "ops.Q8Rows"):
+        """The normed rows in 8 bits, for a product that takes them."""
+        return ops.rmsnorm_q8(x, self.weight, self.eps, out)
+
+    def kernels_needed(self):
+        return self.kernel_modules + (("quant",) if self.rt.int8 else ())
+
     def rms_scale_form(self):
         """``(weight, eps)``: this norm is ``x * weight / sqrt(mean(x^2) + eps)``, one scalar per row times a
         fixed vector.  A matrix product may use that: the scalar commutes with the product, so whoever

@@ -74,3 +74,12 @@ def test_a_weight_is_kept_or_laid_out():
 def test_refusals(make):
     with pytest.raises(ops.KernelError):
         make()
+
+
+def test_what_a_runtime_takes():
+    from skyla_kernel_b200.parts.base import Runtime
+    assert Runtime(torch.device("cpu"), "bfloat16", weights="int8").int8 and not Runtime(torch.device("cpu"), "bfloat16").int8
+    with pytest.raises(ValueError):
+        Runtime(torch.device("cpu"), "float32", weights="int8")
+    with pytest.raises(ValueError):
+        Runtime(torch.device("cpu"), "bfloat16", weights="int4")

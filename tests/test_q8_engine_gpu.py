@@ -1,0 +1,133 @@
+"""Models whose layers' products run in 8 bits (``weights="int8"``): the engine against the plain implementation with the
+same rounding of weights and tokens, in every way of cutting the work."""
+import pytest
+import torch
+
+import plain_q8
+import plain_qwen3 as plain
+from helpers import TINY, make_folder, random_tokens
+
+pytestmark = pytest.mark.gpu
+
+# Of the largest logit, worst and mean.  Where a 16-bit engine rounds what it stores, some tokens' integers come out one
+# step further: that alone moves the plain implementation's logits by up to 5.2e-2 (worst) and 1.05e-2 (mean) on these
+# models (48 sequences, bfloat16 round trips inside the 8-bit run against none).  The limits are about twice that; a
+# fault in a scale, a row or a position moves logits by the order of the largest.
+WORST, MEAN = 0.11, 0.021
+
+
+@pytest.fixture(scope="module")
+def folders(tmp_path_factory):
+    d = tmp_path_factory.mktemp("models")
+    return {n: make_folder(d, n, sharp=1.0) for n in "ABCD"}
+
+
+def _engine(folder, max_tokens=2048, **kw):
+    from skyla_kernel_b200.engine import Engine
+    return Engine.from_folder(folder, max_tokens=max_tokens, weights="int8", **kw)
+
+
+_MODELS = {}
+
+
+def _check(folder, tokens, got, what):
+    if folder not in _MODELS:
+        _MODELS[folder] = plain.read_folder(folder)
+    ref = plain_q8.forward(*_MODELS[folder], tokens)
+    err = (got.cpu() - ref).abs() / ref.abs().max()
+    assert torch.isfinite(got).all() and err.max() <= WORST and err.mean() <= MEAN, \
+        f"{what}: worst {float(err.max()):.3e}, mean {float(err.mean()):.3e}"
+
+
+@pytest.mark.parametrize("name", "ABCD")
+def test_whole_sequences(folders, name):
+    from skyla_kernel_b200.engine import StepItem
+    from skyla_kernel_b200.kernels import ops
+    eng = _engine(folders[name])
+    before = dict(ops.LAUNCHES_BY_MODULE)
+    for n, seed in ((1, 3), (5, 4), (20, 8), (70, 5), (150, 6), (300, 7)):
+        toks = random_tokens(n, TINY[name][0]["vocab_size"], seed)
+        s = eng.alloc_slot()
+        got = eng.step([StepItem(s, toks, list(range(n)))])
+        eng.free_slot(s)
+        _check(folders[name], toks, got, f"{name} n={n}")
+    assert ops.LAUNCHES_BY_MODULE["gemm_q8"] > before.get("gemm_q8", 0) and ops.LAUNCHES_BY_MODULE["quant"] > before.get("quant", 0)
+    assert ops.LAUNCHES_BY_MODULE.get("linear_q8_plain", 0) == before.get("linear_q8_plain", 0)
+    eng.check_errors()
+
+
+@pytest.mark.parametrize("name", "ABCD")
+@pytest.mark.parametrize("graphs", [True, False])
+def test_the_last_32_one_by_one(folders, name, graphs):
+    from skyla_kernel_b200.engine import StepItem
+    eng = _engine(folders[name], cuda_graphs=graphs)
+    toks = random_tokens(100, TINY[name][0]["vocab_size"], 11)
+    s = eng.alloc_slot()
+    rows = [eng.step([StepItem(s, toks[:68], list(range(68)))])]
+    rows += [eng.step([StepItem(s, [t], [0])]) for t in toks[68:]]
+    _check(folders[name], toks, torch.cat(rows), f"{name} one by one")
+    eng.check_errors()
+
+
+@pytest.mark.parametrize("name", "BD")
+def test_unequal_batches(folders, name):
+    """Prompts of unequal length in one step, then a token for each; 20 sequences, so that decode steps leave the kernel
+    that finishes q, k and v itself."""
+    from skyla_kernel_b200.engine import StepItem
+    eng = _engine(folders[name], max_tokens=64 * 64)
+    V = TINY[name][0]["vocab_size"]
+    seqs = [random_tokens(3 + 7 * i % 50 + 6, V, i) for i in range(20)]
+    slots = [eng.alloc_slot() for _ in seqs]
+    got = [[] for _ in seqs]
+    logits = eng.step([StepItem(s, q[:-6], list(range(len(q) - 6))) for s, q in zip(slots, seqs)])
+    at = 0
+    for i, q in enumerate(seqs):
+        got[i].append(logits[at:at + len(q) - 6])
+        at += len(q) - 6
+    for j in range(6):
+        logits = eng.step([StepItem(s, [q[len(q) - 6 + j]], [0]) for s, q in zip(slots, seqs)])
+        for i in range(len(seqs)):
+            got[i].append(logits[i:i + 1])
+    for i in range(0, 20, 3):
+        _check(folders[name], seqs[i], torch.cat(got[i]), f"{name} sequence {i}")
+
+
+def test_generation_through_the_entry_point(folders):
+    import skyla_kernel_b200 as skyla
+    model = skyla.load(folders["D"], weights="int8", max_tokens=4096)
+    V = TINY["D"][0]["vocab_size"]
+    prompts = [random_tokens(n, V, n) for n in (4, 33, 130)]
+    one = model.generate(prompts, max_new_tokens=12, stop_ids=[])
+    assert [len(o) for o in one] == [12] * 3 and all(0 <= t < V for o in one for t in o)
+    assert model.generate(prompts, max_new_tokens=12, stop_ids=[]) == one
+    # every token lies within the limit of what the plain implementation rates highest
+    cfg, w = plain.read_folder(folders["D"])
+    for p, o in zip(prompts, one):
+        logits = plain_q8.forward(cfg, w, list(p) + o[:-1])[len(p) - 1:]
+        gap = logits.max(-1).values - logits.gather(1, torch.tensor(o)[:, None])[:, 0]
+        assert float(gap.max()) <= 2 * WORST * float(logits.abs().max())
+
+
+def test_weights_take_half_the_memory(folders):
+    from skyla_kernel_b200.engine import Engine
+    bf16 = Engine.from_folder(folders["D"])
+    int8 = _engine(folders["D"])
+    head = int8.model.head.weight_bytes() + int8.model.final_norm.weight_bytes()
+    a, b = bf16.weight_bytes() - head, int8.weight_bytes() - head
+    assert 0.5 * a < b < 0.51 * a
+
+
+def test_a_norm_that_knows_nothing_of_8_bits(folders):
+    """Its 16-bit rows are quantised for the products."""
+    from skyla_kernel_b200.engine import StepItem
+    from skyla_kernel_b200.parts.norm import RMSNorm
+    eng = _engine(folders["D"])
+    toks = random_tokens(50, TINY["D"][0]["vocab_size"], 9)
+    forward_rows = RMSNorm.forward_rows
+    try:
+        del RMSNorm.forward_rows
+        s = eng.alloc_slot()
+        got = eng.step([StepItem(s, toks, list(range(50)))])
+    finally:
+        RMSNorm.forward_rows = forward_rows
+    _check(folders["D"], toks, got, "norm without rows")
