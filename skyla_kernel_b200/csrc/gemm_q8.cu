@@ -1120,7 +1120,7 @@ extern "C" int skyla_linear_q8(const void* x, int64_t ldx, const float* x_scale,
   if (M <= 0 || N <= 0) return kOk;
   if (K <= 0 || K > kMaxWidth) return fail(kBadArgument, "linear_q8: K=%d is outside 1..%d", K, kMaxWidth);
   if (mode < kStoreBf16 || mode > kGluBf16) return fail(kBadArgument, "linear_q8: unknown mode %d", mode);
-  if (N > (1 << 30)) return fail(kBadArgument, "linear_q8: %d outputs", N);
+  if (N > (1 << 29) || M > (1 << 29)) return fail(kBadArgument, "linear_q8: %d tokens, %d outputs: at most 2^29", M, N);
   if ((uintptr_t)x % 16 || (uintptr_t)w % 16 || ldx % 16 || ldw % 16)
     return fail(kBadArgument, "linear_q8: rows that do not begin on multiples of 16 bytes");
   const Operands o{x, ldx, w, ldw, mode == kGluBf16 ? 2 * N : N};

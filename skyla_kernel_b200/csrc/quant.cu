@@ -36,6 +36,21 @@ struct Pack {
     if (sizeof(T) == 4) return __uint_as_float(u[i]);
     return __uint_as_float((uint32_t)h[i] << 16);  // a bfloat16 is the upper half of a 32-bit value
   }
+  // the largest of `most` and the elements' magnitudes, as bits of 32-bit values.  (Two 16-bit elements at a time.)
+  __device__ __forceinline__ unsigned largest(unsigned most) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) most = max(most, u[i] & 0x7fffffffu);
+      return most;
+    } else if constexpr (E == 1) {
+      return max(most, (unsigned)(h[0] & 0x7fffu) << 16);
+    } else {
+      unsigned two = 0;
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) two = __vmaxu2(two, u[i] & 0x7fff7fffu);
+      return max(most, max(two << 16, two & 0xffff0000u));
+    }
+  }
   __device__ __forceinline__ void set(int i, float v) {
     if (sizeof(T) == 4) u[i] = __float_as_uint(v);
     else h[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
@@ -48,6 +63,8 @@ __device__ __forceinline__ void store_q(int8_t* p, const uint32_t* n) {
   else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = low_bytes(n);
   else *reinterpret_cast<uint2*>(p) = make_uint2(low_bytes(n), low_bytes(n + 4));
 }
+
+__device__ __constant__ uint32_t kZeros[16] = {};
 
 // The threads of a row: `BLOCK` a block's, else a warp's
 template <bool BLOCK>
@@ -92,25 +109,25 @@ __global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x,
     if (first + j * step < width) kept[j].load(xr + first + j * step);
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
-    if (first + j * step < width) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) most = max(most, abs_bits(kept[j].get(i)));
-    }
+    if (first + j * step < width) most = kept[j].largest(most);
   for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
     Pack<T, E> p;
     p.load(xr + e);
-#pragma unroll
-    for (int i = 0; i < E; ++i) most = max(most, abs_bits(p.get(i)));
+    most = p.largest(most);
   }
   g.meet(most, nullptr);
-  const bool bad = most >= kInfBits;
-  const Step s = step_of(bad ? 0u : most);
+  if (most >= kInfBits) {  // the same for the whole group
+    for (int64_t e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
+    if (g.rank == 0) scale[g.row] = kNan;
+    return;
+  }
+  const Step s = step_of(most);
   auto put = [&](int64_t e, const Pack<T, E>& p) {
     float v[E];
     uint32_t n[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = bad ? 0.f : p.get(i);
-    round_q<E>(v, s, n);
+    for (int i = 0; i < E; ++i) v[i] = p.get(i);
+    round_q<E, sizeof(T) == 2>(v, s, n);
     store_q<E>(qr + e, n);
   };
 #pragma unroll
@@ -121,7 +138,7 @@ __global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x,
     p.load(xr + e);
     put(e, p);
   }
-  if (g.rank == 0) scale[g.row] = bad ? kNan : s.most / kMost;
+  if (g.rank == 0) scale[g.row] = s.most / kMost;
 }
 
 // x += residual (rounded to x's type: the norm is that of the sum as it is kept), then the norm's row in 8 bits.
@@ -187,14 +204,15 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_q8_kernel(TX* __restrict
   }
   g.meet(most, &ss);
   const float inv = 1.0f / sqrtf(ss / (float)width + eps);
-  const bool bad = most >= kInfBits || abs_bits(ss) >= kInfBits || abs_bits(inv) >= kInfBits;
-  const Step s = step_of(bad ? 0u : most);
+  if (most >= kInfBits || abs_bits(ss) >= kInfBits || abs_bits(inv) >= kInfBits) {  // the same for the whole group
+    for (int64_t e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
+    if (g.rank == 0) scale[g.row] = kNan;
+    return;
+  }
+  const Step s = step_of(most);
   auto put = [&](int64_t e, const float* t) {
-    float v[E];
     uint32_t n[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = bad ? 0.f : t[i];
-    round_q<E>(v, s, n);
+    round_q<E, false>(t, s, n);
     store_q<E>(qr + e, n);
   };
 #pragma unroll
@@ -210,7 +228,7 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_q8_kernel(TX* __restrict
     for (int i = 0; i < E; ++i) t[i] = p.get(i) * weight.get(i);
     put(e, t);
   }
-  if (g.rank == 0) scale[g.row] = bad ? kNan : s.most * inv / kMost;
+  if (g.rank == 0) scale[g.row] = s.most * inv / kMost;
 }
 
 template <typename T, int E, bool BLOCK>
@@ -253,16 +271,18 @@ bool rows_on(const void* p, int64_t ld, int size, int bytes) { return (uintptr_t
 
 // How a row is shared out: threads, and loads that each keeps.
 struct Shape { int threads; int keep; bool block; };
-Shape shape_for(int64_t n_rows, int width, int E, int most = 1024) {
+Shape shape_for(int64_t n_rows, int width, int E, int most, int keep) {
   const int64_t loads = ((int64_t)width + E - 1) / E;
-  // a warp a row, eight rows a block
+  // a warp a row, eight or four rows a block
   if (loads <= 32 * 4 && n_rows >= 8) return {256, loads <= 32 ? 1 : 4, false};
-  // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last
-  int64_t threads = n_rows < 592 ? loads : (loads + 3) / 4;
+  if (loads <= 32 * keep && n_rows >= 4096) return {128, keep, false};
+  // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last; many rows: `keep`
+  // loads a thread
+  int64_t threads = n_rows < 592 ? loads : (loads + keep - 1) / keep;
   threads = (threads + 31) / 32 * 32;
   if (threads < 64) threads = 64;
   if (threads > most) threads = most;
-  return {(int)threads, loads <= threads ? 1 : 4, true};
+  return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : keep, true};
 }
 dim3 grid_for(int64_t n_rows, const Shape& s) { return dim3((unsigned)(s.block ? n_rows : (n_rows + s.threads / 32 - 1) / (s.threads / 32))); }
 
@@ -294,9 +314,9 @@ extern "C" int skyla_quantize_rows(const void* x, int x_dtype, int64_t ldx, int6
   SKYLA_DISPATCH(x_dtype, T, {
     constexpr int E = 16 / sizeof(T);
     if (width % E == 0 && rows_on(x, ldx, sizeof(T), 16) && rows_on(q, ldq, 1, E))
-      launch_quantize<T, E>(shape_for(n_rows, width, E), x, ldx, n_rows, width, q, ldq, scale, stream);
+      launch_quantize<T, E>(shape_for(n_rows, width, E, 1024, 4), x, ldx, n_rows, width, q, ldq, scale, stream);
     else
-      launch_quantize<T, 1>(shape_for(n_rows, width, 1), x, ldx, n_rows, width, q, ldq, scale, stream);
+      launch_quantize<T, 1>(shape_for(n_rows, width, 1, 1024, 4), x, ldx, n_rows, width, q, ldq, scale, stream);
   });
   return check_launch("quantize_rows");
 }
@@ -314,12 +334,12 @@ extern "C" int skyla_rmsnorm_q8(void* x, int x_dtype, int64_t ldx, const void* r
     const bool vec = width % E == 0 && rows_on(x, ldx, sizeof(TX), 16) && rows_on(q, ldq, 1, E) && (uintptr_t)weight % 16 == 0 &&
                      (residual == nullptr || rows_on(residual, ldr, r_size, E * r_size < 16 ? E * r_size : 16));
     if (residual == nullptr) {
-      if (vec) launch_norm<TX, float, false, E>(shape_for(n_rows, width, E, kNormThreads), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
-      else launch_norm<TX, float, false, 1>(shape_for(n_rows, width, 1, kNormThreads), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
+      if (vec) launch_norm<TX, float, false, E>(shape_for(n_rows, width, E, kNormThreads, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
+      else launch_norm<TX, float, false, 1>(shape_for(n_rows, width, 1, kNormThreads, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
     } else {
       SKYLA_DISPATCH(r_dtype, TR, {
-        if (vec) launch_norm<TX, TR, true, E>(shape_for(n_rows, width, E, kNormThreads), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
-        else launch_norm<TX, TR, true, 1>(shape_for(n_rows, width, 1, kNormThreads), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
+        if (vec) launch_norm<TX, TR, true, E>(shape_for(n_rows, width, E, kNormThreads, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
+        else launch_norm<TX, TR, true, 1>(shape_for(n_rows, width, 1, kNormThreads, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
       });
     }
   });
@@ -335,7 +355,7 @@ extern "C" int skyla_dequantize_rows(const void* q, int64_t ldq, const float* sc
       launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const int8_t*)q, ldq, scale, n_rows, width, (T*)out, ldo);
     };
     const bool vec = width % 8 == 0 && rows_on(q, ldq, 1, 8) && rows_on(out, ldo, sizeof(T), 16);
-    const Shape s = shape_for(n_rows, width, vec ? 8 : 1);
+    const Shape s = shape_for(n_rows, width, vec ? 8 : 1, 1024, 4);
     if (vec) s.block ? go(dequantize_kernel<T, 8, true>, s) : go(dequantize_kernel<T, 8, false>, s);
     else s.block ? go(dequantize_kernel<T, 1, true>, s) : go(dequantize_kernel<T, 1, false>, s);
   });

@@ -608,6 +608,9 @@ def q8_rows(n: int, width: int, device) -> Q8Rows:
     return Q8Rows(q if q.shape[1] == width else q[:, :width], torch.empty(n, dtype=torch.float32, device=device))
 
 
+_MOST = 1 << 29  # rows or elements of a row: the launchers count them in 32 bits
+
+
 def _dims(t: torch.Tensor, what: str):
     """(rows, width, row stride) of a 2-D tensor whose rows are contiguous."""
     if t.dim() != 2:
@@ -616,6 +619,8 @@ def _dims(t: torch.Tensor, what: str):
     ld, step = t.stride()
     if step != 1 and width > 1:
         raise KernelError(f"{what}: expected contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
+    if n > _MOST or width > _MOST:
+        raise KernelError(f"{what}: {n} rows of {width}: at most 2^29 of either")
     return n, width, ld if n > 1 else max(ld, width)
 
 
@@ -711,7 +716,8 @@ def dequantize_rows(rows: Q8Rows, out: torch.Tensor) -> torch.Tensor:
 def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[Q8Rows] = None,
                residual: Optional[torch.Tensor] = None) -> Q8Rows:
     """``rmsnorm(x) * weight`` in 8-bit rows, computed in 32 bits; with ``residual`` the rows are added into ``x``
-    first (``x`` is written, in its own type, and the norm is that of the sum as it is kept).
+    first (``x`` is written, in its own type, and the norm is that of the sum as it is kept).  ``residual`` is ``x``
+    itself or lies apart from it.
 
     ``x`` and ``residual``: bfloat16 or float32.  A row whose sum of squares or whose products with the weight
     leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row of zeros with ``eps = 0``."""
@@ -745,8 +751,8 @@ class Q8Weight:
 
     ``gated``: all gate rows, then the up rows of the same outputs.  The tensors are kept as they are if the rows
     begin on multiples of 16 bytes, else copied into such rows.  The product's kernels ask for the weight before
-    they wait for the kernels ahead of them, so it is finished for good: the constructor waits for the current
-    stream, and nobody writes the tensors afterwards."""
+    they wait for the kernels ahead of them, so it is finished for good: the constructor waits for the device (and
+    refuses to run inside a stream capture), and nobody writes the tensors afterwards."""
 
     __slots__ = ("rows", "gated", "n_out", "n_in", "ld")
 
@@ -756,12 +762,14 @@ class Q8Weight:
             raise KernelError(f"Q8Weight: {width} inputs are outside 1..{Q8_MAX_WIDTH}")
         if n < 1 or (gated and n % 2):
             raise KernelError(f"Q8Weight: {n} rows" + (" do not divide into gate and up" if gated else ""))
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise KernelError("Q8Weight: a weight is laid out before a stream is captured, not inside")
         if ld % 16 or ld < width or q.data_ptr() % 16:
             kept = q8_rows(n, width, q.device).q
             kept.copy_(q)
             q, ld = kept, _dims(kept, "Q8Weight")[2]
         if q.is_cuda:
-            torch.cuda.current_stream(q.device).synchronize()
+            torch.cuda.synchronize(q.device)
         self.rows, self.gated, self.n_in, self.ld = Q8Rows(q, scale), bool(gated), width, ld
         self.n_out = n // 2 if gated else n
 
@@ -801,13 +809,14 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
     if code != (F32 if mode == ACCUMULATE else BF16 if mode == GATED else code):
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
-    dev = _device_of(q, scale, rows.q, rows.scale, y)
+    flag = _state(state, y).error_flag if y.is_cuda else y
+    dev = _device_of(q, scale, rows.q, rows.scale, y, flag)
     if m == 1:
         ldx = w.ld  # the distance to a next row that is not there
     if ldx % 16 == 0 and ldx >= k and q.data_ptr() % 16 == 0:
         epilogue = TC_ACCUM_F32 if mode == ACCUMULATE else TC_GLU_BF16 if mode == GATED else TC_STORE_F32 if code == F32 else TC_STORE_BF16
         _linear_q8(dev, q.data_ptr(), ldx, scale.data_ptr(), rows.q.data_ptr(), w.ld, rows.scale.data_ptr(), m, yn, k, y.data_ptr(), ldy,
-                   epilogue, _state(state, y).error_flag.data_ptr())
+                   epilogue, flag.data_ptr())
     else:
         _linear_q8_plain(dev, q.data_ptr(), ldx, scale.data_ptr(), rows.q.data_ptr(), w.ld, rows.scale.data_ptr(), m, yn, k, y.data_ptr(),
                          code, ldy, mode)

@@ -66,6 +66,9 @@ def test_a_weight_is_kept_or_laid_out():
     lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 4, dtype=torch.bfloat16), ops.ACCUMULATE),
     lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(2, 4), 7),
     lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 16)), torch.zeros(1, 4).expand(2, 4)),
+    # sizes that the launchers cannot count
+    lambda: ops.quantize_rows(torch.empty(1, 2 ** 31, device="meta")),
+    lambda: ops.quantize_rows(torch.empty(2 ** 31, 1, device="meta")),
     # all of them on the host
     lambda: ops.quantize_rows(torch.zeros(2, 3)),
     lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), 1e-6),
@@ -74,6 +77,12 @@ def test_a_weight_is_kept_or_laid_out():
 def test_refusals(make):
     with pytest.raises(ops.KernelError):
         make()
+
+
+def test_too_many_elements_are_named():
+    for shape in ((1, 2 ** 31), (2 ** 31, 2)):
+        with pytest.raises(ops.KernelError, match="2\\^29"):
+            ops.rmsnorm_q8(torch.empty(*shape, device="meta"), torch.empty(shape[1], device="meta"), 1e-6)
 
 
 def test_what_a_runtime_takes():

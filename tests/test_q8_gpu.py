@@ -64,6 +64,23 @@ def test_quotients_that_end_in_one_half():
     assert torch.equal(got.q, q) and torch.equal(got.scale, scale)
 
 
+def test_every_bfloat16_value_against_every_largest():
+    """Rows of all 16-bit values up to their largest, for every significand that a largest can have."""
+    sig = torch.arange(128, 256, dtype=F32)                                # significands
+    values = torch.cat([sig * 2.0 ** e for e in range(-10, 1)])            # nearer to 0 than A / 254 all quotients round to 0
+    for lo in range(128, 256, 16):
+        rows = []
+        for a in range(lo, lo + 16):
+            rows.append(torch.where(values <= a, values, torch.full_like(values, -a)))
+            rows[-1][-1] = a
+        x = torch.stack(rows).to(BF16).to(DEV)
+        assert torch.equal(x.float().amax(1).cpu(), torch.arange(lo, lo + 16).float())
+        for t in (x, x * 2.0 ** -100):
+            q, scale = _want(t)
+            got = ops.quantize_rows(t)
+            assert torch.equal(got.q, q) and torch.equal(got.scale, scale)
+
+
 def test_rows_of_zeros_small_numbers_and_nans():
     w = 40
     x = _rand(9, w, seed=3)
@@ -238,6 +255,59 @@ def test_a_row_without_a_scale_spoils_itself_only(m):
     bad[m // 2] = True
     assert torch.isnan(y[bad]).all() and torch.equal(y[~bad], _values(x, w)[~bad])
     assert ops.linear_q8(ops.Q8Rows(x.q[:0], x.scale[:0]), w, y[:0]).shape == (0, 64)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 100, 129, 300])
+@pytest.mark.parametrize("n", [64, 203])
+def test_a_product_writes_its_rows_only(m, n):
+    """y as the middle of a larger buffer: what lies before, behind and between stays."""
+    x = ops.quantize_rows(_rand(m, 512, seed=1))
+    for dtype, mode, gated in ((F32, ops.STORE, False), (BF16, ops.STORE, False), (F32, ops.ACCUMULATE, False), (BF16, ops.GATED, True)):
+        w = ops.Q8Weight.quantize(_rand(2 * n if gated else n, 512, seed=2), gated=gated)
+        whole = torch.full((m + 4, n + 13 if n % 2 else n + 16), 3.0, dtype=dtype, device=DEV)
+        before = whole.clone()
+        ops.linear_q8(x, w, whole[2:m + 2, :n], mode)
+        assert not torch.equal(whole[2:m + 2, :n], before[2:m + 2, :n])
+        whole[2:m + 2, :n] = 3
+        assert torch.equal(whole, before), (dtype, mode)
+
+
+def test_many_tokens_of_a_narrow_product():
+    """More tiles of tokens than a launch has blocks, offsets beyond 2^31 bytes of y."""
+    m, k, n = 300000, 16, 2048
+    q = torch.randint(-127, 128, (m, k), dtype=torch.int8, device=DEV)
+    x = ops.Q8Rows(q, torch.full((m,), 0.5, device=DEV))
+    w = ops.Q8Weight(torch.randint(-127, 128, (n, k), dtype=torch.int8, device=DEV), torch.full((n,), 0.25, device=DEV))
+    y = ops.linear_q8(x, w, torch.empty(m, n, device=DEV))
+    for lo in (0, 149990, m - 200):
+        rows = ops.Q8Rows(q[lo:lo + 200], x.scale[lo:lo + 200])
+        assert torch.equal(y[lo:lo + 200], _values(rows, w))
+
+
+def test_long_rows_apart_beyond_32_bits():
+    """Rows 2^30 elements apart: offsets of 2^32 bytes and more."""
+    apart, width = 1 << 30, 1000
+    x = torch.empty(2 * apart + width, dtype=BF16, device=DEV).as_strided((3, width), (apart, 1))
+    x.copy_(_rand(3, width, seed=5))
+    got = ops.quantize_rows(x)
+    q, scale = _want(x)
+    assert torch.equal(got.q, q) and torch.equal(got.scale, scale)
+    weight = torch.ones(width, device=DEV)
+    got = ops.rmsnorm_q8(x, weight, 1e-6, residual=x)
+    _norm_close(x, weight, 1e-6, got)
+
+
+def test_a_weight_is_not_laid_out_inside_a_capture():
+    w = _rand(64, 64)
+    ops.Q8Weight.quantize(w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows = ops.quantize_rows(w)
+        with pytest.raises(ops.KernelError):
+            ops.Q8Weight(*rows)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(rows.q, _want(w)[0])
 
 
 def test_a_weight_of_the_first_outputs():
