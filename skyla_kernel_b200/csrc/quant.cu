@@ -9,7 +9,6 @@ using namespace skyla::q8;
 SKYLA_EXPORT_ERROR_MESSAGE()
 
 namespace {
-constexpr int kNormThreads = 512;  // most threads of a norm's block: they hold 32-bit products, twice what a row's bfloat16 takes
 
 template <int BYTES> struct Word;
 template <> struct Word<1> { typedef uint8_t type; };
@@ -93,7 +92,7 @@ struct Group {
 };
 
 template <typename T, int E, int kKeep, bool BLOCK>
-__global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t n_rows, int width, int8_t* __restrict__ q,
+__global__ void __launch_bounds__(kKeep == 8 ? 512 : 1024) quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t n_rows, int width, int8_t* __restrict__ q,
                                 int64_t ldq, float* __restrict__ scale) {
   allow_dependents();
   grid_dependency_wait();
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x,
 // = 127 t / A: the integers do not depend on inv, which goes into the scale alone, so the sum of squares and the largest
 // t are found in one pass and one meeting.
 template <typename TX, typename TR, bool ADD, int E, int kKeep, bool BLOCK>
-__global__ void __launch_bounds__(kNormThreads) rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int64_t n_rows,
+__global__ void __launch_bounds__(kKeep == 1 ? 1024 : 512) rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int64_t n_rows,
                                   int width, const float* __restrict__ w, float eps, int8_t* __restrict__ q, int64_t ldq,
                                   float* __restrict__ scale) {
   allow_dependents();
@@ -203,8 +202,8 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_q8_kernel(TX* __restrict
     take(e, p, add, weight, t);
   }
   g.meet(most, &ss);
-  const float inv = 1.0f / sqrtf(ss / (float)width + eps);
-  if (most >= kInfBits || abs_bits(ss) >= kInfBits || abs_bits(inv) >= kInfBits) {  // the same for the whole group
+  // the same for the whole group (the mean square and eps may both be zero; the scale is one thread's work)
+  if (most >= kInfBits || abs_bits(ss) >= kInfBits || (eps == 0.f && ss / (float)width == 0.f)) {
     for (int64_t e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
     if (g.rank == 0) scale[g.row] = kNan;
     return;
@@ -228,7 +227,7 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_q8_kernel(TX* __restrict
     for (int i = 0; i < E; ++i) t[i] = p.get(i) * weight.get(i);
     put(e, t);
   }
-  if (g.rank == 0) scale[g.row] = s.most * inv / kMost;
+  if (g.rank == 0) scale[g.row] = s.most * (1.0f / sqrtf(ss / (float)width + eps)) / kMost;
 }
 
 template <typename T, int E, bool BLOCK>
@@ -269,20 +268,22 @@ int check_sizes(const char* what, int64_t n_rows, int width, int64_t ld_in, int6
 // Rows of `size`-byte elements that begin on multiples of `bytes`
 bool rows_on(const void* p, int64_t ld, int size, int bytes) { return (uintptr_t)p % bytes == 0 && ld * size % bytes == 0; }
 
-// How a row is shared out: threads, and loads that each keeps.
+// How a row is shared out: threads, and loads that each keeps.  Four loads a thread where there are many rows: what a thread
+// does once for its row, some 200 instructions, counts for that many, and more registers a thread cost more than that gives
+// (8,192 x 4,096 with its residual: 74 / 59 / 80 us at two / four / eight loads).  Only the quantisation of long rows
+// (`most_kept` 8), whose loads stay as they come, gains by eight (2,048 x 12,288 of 32 bits: 35 to 28 us).
 struct Shape { int threads; int keep; bool block; };
-Shape shape_for(int64_t n_rows, int width, int E, int most, int keep) {
+Shape shape_for(int64_t n_rows, int width, int E, int most_kept) {
   const int64_t loads = ((int64_t)width + E - 1) / E;
-  // a warp a row, eight or four rows a block
+  // a warp a row, eight rows a block
   if (loads <= 32 * 4 && n_rows >= 8) return {256, loads <= 32 ? 1 : 4, false};
-  if (loads <= 32 * keep && n_rows >= 4096) return {128, keep, false};
-  // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last; many rows: `keep`
-  // loads a thread
-  int64_t threads = n_rows < 592 ? loads : (loads + keep - 1) / keep;
-  threads = (threads + 31) / 32 * 32;
-  if (threads < 64) threads = 64;
-  if (threads > most) threads = most;
-  return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : keep, true};
+  // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last
+  int64_t threads = n_rows < 592 && loads <= 1024 ? loads : (loads + 3) / 4;
+  if (n_rows < 592 && loads > 1024) threads = 512;
+  if (n_rows >= 592 && threads > 512) threads = (loads + most_kept - 1) / most_kept;
+  if (threads > 512 && loads > 1024) threads = 512;
+  threads = threads < 64 ? 64 : (threads + 31) / 32 * 32;
+  return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : most_kept, true};
 }
 dim3 grid_for(int64_t n_rows, const Shape& s) { return dim3((unsigned)(s.block ? n_rows : (n_rows + s.threads / 32 - 1) / (s.threads / 32))); }
 
@@ -292,7 +293,7 @@ void launch_quantize(const Shape& s, const void* x, int64_t ldx, int64_t n_rows,
   auto go = [&](auto kernel) {
     launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const T*)x, ldx, n_rows, width, (int8_t*)q, ldq, scale);
   };
-  if (s.block) s.keep == 1 ? go(quantize_kernel<T, E, 1, true>) : go(quantize_kernel<T, E, 4, true>);
+  if (s.block) s.keep == 1 ? go(quantize_kernel<T, E, 1, true>) : s.keep == 4 ? go(quantize_kernel<T, E, 4, true>) : go(quantize_kernel<T, E, 8, true>);
   else s.keep == 1 ? go(quantize_kernel<T, E, 1, false>) : go(quantize_kernel<T, E, 4, false>);
 }
 template <typename TX, typename TR, bool ADD, int E>
@@ -314,9 +315,9 @@ extern "C" int skyla_quantize_rows(const void* x, int x_dtype, int64_t ldx, int6
   SKYLA_DISPATCH(x_dtype, T, {
     constexpr int E = 16 / sizeof(T);
     if (width % E == 0 && rows_on(x, ldx, sizeof(T), 16) && rows_on(q, ldq, 1, E))
-      launch_quantize<T, E>(shape_for(n_rows, width, E, 1024, 4), x, ldx, n_rows, width, q, ldq, scale, stream);
+      launch_quantize<T, E>(shape_for(n_rows, width, E, 8), x, ldx, n_rows, width, q, ldq, scale, stream);
     else
-      launch_quantize<T, 1>(shape_for(n_rows, width, 1, 1024, 4), x, ldx, n_rows, width, q, ldq, scale, stream);
+      launch_quantize<T, 1>(shape_for(n_rows, width, 1, 8), x, ldx, n_rows, width, q, ldq, scale, stream);
   });
   return check_launch("quantize_rows");
 }
@@ -334,12 +335,12 @@ extern "C" int skyla_rmsnorm_q8(void* x, int x_dtype, int64_t ldx, const void* r
     const bool vec = width % E == 0 && rows_on(x, ldx, sizeof(TX), 16) && rows_on(q, ldq, 1, E) && (uintptr_t)weight % 16 == 0 &&
                      (residual == nullptr || rows_on(residual, ldr, r_size, E * r_size < 16 ? E * r_size : 16));
     if (residual == nullptr) {
-      if (vec) launch_norm<TX, float, false, E>(shape_for(n_rows, width, E, kNormThreads, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
-      else launch_norm<TX, float, false, 1>(shape_for(n_rows, width, 1, kNormThreads, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
+      if (vec) launch_norm<TX, float, false, E>(shape_for(n_rows, width, E, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
+      else launch_norm<TX, float, false, 1>(shape_for(n_rows, width, 1, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
     } else {
       SKYLA_DISPATCH(r_dtype, TR, {
-        if (vec) launch_norm<TX, TR, true, E>(shape_for(n_rows, width, E, kNormThreads, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
-        else launch_norm<TX, TR, true, 1>(shape_for(n_rows, width, 1, kNormThreads, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
+        if (vec) launch_norm<TX, TR, true, E>(shape_for(n_rows, width, E, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
+        else launch_norm<TX, TR, true, 1>(shape_for(n_rows, width, 1, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
       });
     }
   });
@@ -355,7 +356,7 @@ extern "C" int skyla_dequantize_rows(const void* q, int64_t ldq, const float* sc
       launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const int8_t*)q, ldq, scale, n_rows, width, (T*)out, ldo);
     };
     const bool vec = width % 8 == 0 && rows_on(q, ldq, 1, 8) && rows_on(out, ldo, sizeof(T), 16);
-    const Shape s = shape_for(n_rows, width, vec ? 8 : 1, 1024, 4);
+    const Shape s = shape_for(n_rows, width, vec ? 8 : 1, 4);
     if (vec) s.block ? go(dequantize_kernel<T, 8, true>, s) : go(dequantize_kernel<T, 8, false>, s);
     else s.block ? go(dequantize_kernel<T, 1, true>, s) : go(dequantize_kernel<T, 1, false>, s);
   });
