@@ -453,6 +453,116 @@ __device__ __forceinline__ void put16(uint32_t row_smem, int row, int c, uint32_
                ::"r"(row_smem + (uint32_t)((c ^ (row & 7)) << 4)), "r"(a), "r"(b), "r"(d), "r"(e) : "memory");
 }
 
+// The epilogue of a tile: the chunks first, first + step, ... of its outputs (32 of 32-bit, 64 of bfloat16), from the
+// accumulator's columns as `columns16(column, registers)` brings sixteen of them for this thread's token.
+template <int MODE, int BF, typename Columns>
+__device__ __forceinline__ void drain(const Args& a, const CUtensorMap* map_y, int by_tma, const float* ws, float xs, int f0, int tok0,
+                                      int quad, int lane, bool sender, uint32_t out_smem, int& n_sent, int first, int step,
+                                      volatile int& abort_flag, Columns columns16) {
+  constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
+  constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
+  constexpr int kCols = f32 ? 32 : (kTileOutputs < 64 ? kTileOutputs : 64);  // outputs of a buffer's rows
+  constexpr int kChunks = kTileOutputs / kCols;
+  const int row = quad * 32 + lane;
+  // 32 columns at a time: values of this thread's token
+  auto values = [&](int c0, float* v) {
+    uint32_t r[32];
+    __syncwarp();
+    columns16(c0, r);
+    columns16(c0 + 16, r + 16);
+    if (MODE == kGluBf16) {
+      uint32_t u[32];
+      columns16(BF / 2 + c0, u);
+      columns16(BF / 2 + c0 + 16, u + 16);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        v[j] = silu_times(scaled((int)r[j], xs, ws[c0 + j]), scaled((int)u[j], xs, ws[BF / 2 + c0 + j]));
+    } else {
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = scaled((int)r[j], xs, ws[c0 + j]);
+    }
+  };
+#pragma unroll 1
+  for (int chunk = first; chunk < kChunks; chunk += step) {
+    const int c0 = chunk * kCols;
+    if (f0 + c0 >= a.N) break;  // the same for all four warps
+    const uint32_t out = out_smem + (uint32_t)(n_sent & 1) * kOutBytes;
+    // who read this buffer last (two chunks ago) must be done with it: the send, or, row by row, the warps, which have
+    // met since
+    if (by_tma && sender) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
+    const uint32_t row_smem = out + (uint32_t)row * 128u;
+#pragma unroll
+    for (int h = 0; h < kCols / 32; ++h) {
+      float v[32];
+      values(c0 + 32 * h, v);
+      if (f32) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          put16(row_smem, row, c, __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]),
+                __float_as_uint(v[4 * c + 3]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          put16(row_smem, row, 4 * h + c, pack_bf16(v[8 * c], v[8 * c + 1]), pack_bf16(v[8 * c + 2], v[8 * c + 3]),
+                pack_bf16(v[8 * c + 4], v[8 * c + 5]), pack_bf16(v[8 * c + 6], v[8 * c + 7]));
+      }
+    }
+    if (by_tma) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the TMA unit reads what the threads wrote
+    asm volatile("barrier.sync 1, 128;" ::: "memory");
+    if (by_tma) {
+      if (sender && !abort_flag) {
+        if (MODE == kAccumF32)
+          asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+                       ::"l"(map_y), "r"(out), "r"(f0 + c0), "r"(tok0) : "memory");
+        else
+          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                       ::"l"(map_y), "r"(out), "r"(f0 + c0), "r"(tok0) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else {
+      // a warp takes 32 rows, one after the other, its lanes neighbouring outputs.  (Compact code: a launch starts with
+      // cold instruction caches.  Eight rows at a time, pairs of bfloat16 in one store: 333 tokens x 2,561 to 1,111 took
+      // 10.4 instead of 8.7 us.)
+#pragma unroll 4
+      for (int i = 0; i < 32; ++i) {
+        const int r = quad * 32 + i;
+        if (tok0 + r >= a.M) break;
+        const int64_t at = (int64_t)(tok0 + r) * a.ldy + f0 + c0;
+#pragma unroll
+        for (int h = 0; h < kCols / 32; ++h) {
+          const int c = lane + 32 * h;
+          const uint32_t from = out + (uint32_t)r * 128u +
+                                (uint32_t)((((c * (f32 ? 4 : 2)) >> 4) ^ (r & 7)) << 4) + (uint32_t)((c * (f32 ? 4 : 2)) & 15);
+          if (f0 + c0 + c >= a.N) continue;
+          if (f32) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+            float* y = (float*)a.y + at + c;
+            *y = MODE == kAccumF32 ? __fadd_rn(*y, v) : v;
+          } else {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+            ((uint16_t*)a.y)[at + c] = v;
+          }
+        }
+      }
+    }
+    ++n_sent;
+  }
+}
+
+// The scales of a tile's columns, by the 128 threads of the epilogue.
+template <int MODE, int BF>
+__device__ __forceinline__ void tile_scales(const Args& a, float* ws, int f0, int et) {
+  for (int c = et; c < BF; c += 128) {
+    const int f = MODE == kGluBf16 ? f0 + c % (BF / 2) : f0 + c;
+    ws[c] = f < a.N ? a.w_scale[MODE == kGluBf16 && c >= BF / 2 ? a.N + f : f] : 0.f;
+  }
+}
+
 struct TileArgs {
   int by_tma;         // map_y is y's: outputs leave by TMA
   int boxes;          // the maps of x and w bring a stage's K blocks at once (K in whole blocks); else one by one
@@ -469,7 +579,6 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   using C = TileCfg<MODE, BF>;
   constexpr int kStages = C::kStages;
   constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
-  constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint32_t tmem_base_slot;
   __shared__ volatile int abort_flag;
@@ -615,10 +724,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       const int f_tile = tile / ta.n_t_tiles, t_tile = tile % ta.n_t_tiles;
       const int tok0 = t_tile * BM, tok = tok0 + row, f0 = f_tile * kTileOutputs;
       asm volatile("barrier.sync 1, 128;" ::: "memory");  // the last tile's scales have been read
-      for (int c = et; c < BF; c += 128) {
-        const int f = MODE == kGluBf16 ? f0 + c % (BF / 2) : f0 + c;
-        ws[c] = f < a.N ? a.w_scale[MODE == kGluBf16 && c >= BF / 2 ? a.N + f : f] : 0.f;
-      }
+      tile_scales<MODE, BF>(a, ws, f0, et);
       if (!waited) grid_dependency_wait();
       waited = true;
       const float xs = tok < a.M ? a.x_scale[tok] : 0.f;
@@ -672,97 +778,8 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           tmem_ld16(taddr + c0, r);
         }
       };
-      // 32 columns at a time: values of this thread's token
-      auto values = [&](int c0, float* v) {
-        uint32_t r[32];
-        __syncwarp();
-        columns16(c0, r);
-        columns16(c0 + 16, r + 16);
-        if (MODE == kGluBf16) {
-          uint32_t u[32];
-          columns16(BF / 2 + c0, u);
-          columns16(BF / 2 + c0 + 16, u + 16);
-          if (!SPLIT) tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = silu_times(scaled((int)r[j], xs, ws[c0 + j]), scaled((int)u[j], xs, ws[BF / 2 + c0 + j]));
-        } else {
-          if (!SPLIT) tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = scaled((int)r[j], xs, ws[c0 + j]);
-        }
-      };
-      constexpr int kCols = f32 ? 32 : (kTileOutputs < 64 ? kTileOutputs : 64);  // outputs of a buffer's rows
-      constexpr int kChunks = kTileOutputs / kCols;
-      // a split's block finishes every ta.splits-th chunk
-#pragma unroll 1
-      for (int chunk = rank; chunk < kChunks; chunk += SPLIT ? ta.splits : 1) {
-        const int c0 = chunk * kCols;
-        if (f0 + c0 >= a.N) break;  // the same for all four warps
-        const uint32_t out = out_smem + (uint32_t)(n_sent & 1) * kOutBytes;
-        // who read this buffer last (two chunks ago) must be done with it: the send, or, row by row, the warps, which
-        // have met since
-        if (ta.by_tma && sender) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        asm volatile("barrier.sync 1, 128;" ::: "memory");
-        const uint32_t row_smem = out + (uint32_t)row * 128u;
-#pragma unroll
-        for (int h = 0; h < kCols / 32; ++h) {
-          float v[32];
-          values(c0 + 32 * h, v);
-          if (f32) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              put16(row_smem, row, c, __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]),
-                    __float_as_uint(v[4 * c + 3]));
-          } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              put16(row_smem, row, 4 * h + c, pack_bf16(v[8 * c], v[8 * c + 1]), pack_bf16(v[8 * c + 2], v[8 * c + 3]),
-                    pack_bf16(v[8 * c + 4], v[8 * c + 5]), pack_bf16(v[8 * c + 6], v[8 * c + 7]));
-          }
-        }
-        if (ta.by_tma) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the TMA unit reads what the threads wrote
-        asm volatile("barrier.sync 1, 128;" ::: "memory");
-        if (ta.by_tma) {
-          if (sender && (!SPLIT || !abort_flag)) {
-            if (MODE == kAccumF32)
-              asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
-                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(tok0) : "memory");
-            else
-              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
-                           ::"l"(&map_y), "r"(out), "r"(f0 + c0), "r"(tok0) : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else {
-          // a warp takes 32 rows, one after the other, its lanes neighbouring outputs.  (Compact code: a launch starts
-          // with cold instruction caches.  Eight rows at a time, pairs of bfloat16 in one store: 333 tokens x 2,561 to
-          // 1,111 took 10.4 instead of 8.7 us.)
-#pragma unroll 4
-          for (int i = 0; i < 32; ++i) {
-            const int r = quad * 32 + i;
-            if (tok0 + r >= a.M) break;
-            const int64_t at = (int64_t)(tok0 + r) * a.ldy + f0 + c0;
-#pragma unroll
-            for (int h = 0; h < kCols / 32; ++h) {
-              const int c = lane + 32 * h;
-              const uint32_t from = out + (uint32_t)r * 128u +
-                                    (uint32_t)((((c * (f32 ? 4 : 2)) >> 4) ^ (r & 7)) << 4) + (uint32_t)((c * (f32 ? 4 : 2)) & 15);
-              if (f0 + c0 + c >= a.N) continue;
-              if (f32) {
-                float v;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
-                float* y = (float*)a.y + at + c;
-                *y = MODE == kAccumF32 ? __fadd_rn(*y, v) : v;
-              } else {
-                uint16_t v;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-                ((uint16_t*)a.y)[at + c] = v;
-              }
-            }
-          }
-        }
-        ++n_sent;
-      }
+      drain<MODE, BF>(a, &map_y, ta.by_tma, ws, xs, f0, tok0, quad, lane, sender, out_smem, n_sent, rank, SPLIT ? ta.splits : 1, abort_flag,
+                      columns16);
       // this warp has read its lanes of the accumulator: hand it back to the MMA warp
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -799,6 +816,191 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)C::kTmemCols) : "memory");
   }
+}
+
+// ---------------------------------------------------------------------------------- many tokens, two SMs a tile
+// The same work for products of many tiles: a cluster of two blocks takes tiles of 256 tokens x 256 columns with
+// tcgen05's cta_group::2.  Each block holds its 128 tokens and HALF of the columns' weight rows (a gated weight: the
+// first block the gate rows, the second the up rows); the instruction, issued by the first block, reads both blocks'
+// shared memory and leaves each block its own tokens' accumulator.  So a K block brings 32 KB into an SM where
+// q8_tile_kernel brings 48.  Both blocks' loads count into the first block's barrier; its commits free the stage, and
+// hand over the accumulator, in both.
+constexpr int kPairStageBytes = 2 * BM * KB;  // 128 tokens and 128 weight rows
+constexpr int kPairStages = 6;
+constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 2 * kOutBytes + 1024 + 256;
+static_assert(kPairSmemBytes + 256 * 4 + 64 <= 227 * 1024, "shared memory of a block");
+
+__device__ __forceinline__ uint32_t on_first(uint32_t addr) {  // the same place in the cluster's first block
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {  // to the barrier at this place in both blocks
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+q8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ CUtensorMap map_y, const Args a, const TileArgs ta) {
+  constexpr int BF = 256, kStages = kPairStages;
+  constexpr int kTileOutputs = MODE == kGluBf16 ? BF / 2 : BF;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ __align__(16) float ws[BF];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t out_smem = base + kStages * kPairStageBytes;
+  const uint32_t bars = out_smem + 2 * kOutBytes;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kStages + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kStages + 2 + b); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int total_kb = (a.K + KB - 1) / KB;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);   // (in the first block) its loader, which expects both blocks' bytes
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), 8);  // (in the first block) one arrival per epilogue warp of both
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  // both blocks' barriers and accumulators exist from here on
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_base_slot;
+  allow_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int kbg = 0;
+      bool ok = true, waited = false;
+      for (int tile = first; ok && tile < ta.n_tiles; tile += step) {
+        const int f_tile = tile / ta.n_t_tiles, t_tile = tile % ta.n_t_tiles;
+        const int w_row = f_tile * kTileOutputs + (rank == 0 ? 0 : MODE == kGluBf16 ? a.N : BM);
+        const int x_row = (2 * t_tile + (int)rank) * BM;
+        auto load_weights = [&](int kb, int s) {
+          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kPairStageBytes);
+          tma_load_2d_pair(base + s * kPairStageBytes + BM * KB, &map_w, on_first(full_bar(s)), kb * KB, w_row);
+        };
+        // weights are finished before any launch that reads them
+        const int n_pre = waited ? 0 : min(kStages, total_kb);
+        for (int i = 0; i < n_pre; ++i) load_weights(i, i);
+        if (!waited) grid_dependency_wait();
+        waited = true;
+        for (int kb = 0; kb < total_kb; ++kb, ++kbg) {
+          const int s = kbg % kStages;
+          if (kbg >= n_pre) {
+            if (!mbar_wait(empty_bar(s), ((kbg / kStages) & 1) ^ 1, &abort_flag, a.error_flag, 1)) { ok = false; break; }
+            load_weights(kb, s);
+          }
+          tma_load_2d_pair(base + s * kPairStageBytes, &map_x, on_first(full_bar(s)), kb * KB, x_row);
+        }
+      }
+      if (!ok) {  // gave up: give the loads in flight, which count into the first block's barriers, time to land
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = (idesc_i8(BF) & ~(0x1fu << 24)) | ((256u >> 4) << 24);  // M = 256
+      int kbg = 0, it = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < ta.n_tiles; tile += step, ++it) {
+        const int buf = it & 1;
+        if (!mbar_wait(acc_empty_bar(buf), ((it >> 1) & 1) ^ 1, &abort_flag, a.error_flag, 5)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem_base + buf * BF;
+        for (int kb = 0; kb < total_kb; ++kb, ++kbg) {
+          const int s = kbg % kStages;
+          if (!mbar_wait(full_bar(s), (kbg / kStages) & 1, &abort_flag, a.error_flag, 2)) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t sx = base + s * kPairStageBytes;
+          const uint64_t dx = umma_desc(sx), dw = umma_desc(sx + BM * KB);
+#pragma unroll
+          for (int k = 0; k < KB / 32; ++k) {
+            const uint32_t accumulate = (kb > 0 || k > 0) ? 1u : 0u;
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "setp.ne.b32 p, %4, 0;\n\t"
+                "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                ::"r"(d), "l"(dx + 2 * k), "l"(dw + 2 * k), "r"(idesc), "r"(accumulate) : "memory");
+          }
+          umma_commit_pair(empty_bar(s));
+        }
+        umma_commit_pair(acc_full_bar(buf));
+      }
+    }
+  } else {
+    const int quad = warp & 3, row = quad * 32 + lane, et = threadIdx.x - 64;
+    const bool sender = warp == 2 && lane == 0;
+    int n_sent = 0, it = 0;
+    bool waited = false;
+    for (int tile = first; tile < ta.n_tiles; tile += step, ++it) {
+      const int buf = it & 1;
+      const int f_tile = tile / ta.n_t_tiles, t_tile = tile % ta.n_t_tiles;
+      const int tok0 = (2 * t_tile + (int)rank) * BM, tok = tok0 + row, f0 = f_tile * kTileOutputs;
+      asm volatile("barrier.sync 1, 128;" ::: "memory");  // the last tile's scales have been read
+      tile_scales<MODE, BF>(a, ws, f0, et);
+      if (!waited) grid_dependency_wait();
+      waited = true;
+      const float xs = tok < a.M ? a.x_scale[tok] : 0.f;
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
+      if (!mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t taddr = tmem_base + buf * BF + ((uint32_t)(quad * 32) << 16);
+      if (tok0 < a.M)  // the same for the block
+        drain<MODE, BF>(a, &map_y, ta.by_tma, ws, xs, f0, tok0, quad, lane, sender, out_smem, n_sent, 0, 1, abort_flag,
+                        [&](int c0, uint32_t* r) { tmem_ld16(taddr + c0, r); });
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(on_first(acc_empty_bar(buf))) : "memory");
+    }
+    if (ta.by_tma && sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  if (warp == 1 && lane == 0) {  // every accumulator must be idle before its columns are freed
+    const int my_tiles = first < ta.n_tiles ? (ta.n_tiles - first + step - 1) / step : 0;
+    for (int b = 0; b < 2; ++b) {
+      const int uses = (my_tiles + 1 - b) / 2;
+      if (uses > 0) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(acc_full_bar(b), (uses - 1) & 1) && clock64() - t0 < kWaitCycles) {}
+      }
+    }
+  }
+  // neither block leaves while the other may read its shared memory, or count into its barriers
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -992,7 +1194,33 @@ int launch_rows(const Operands& o, const Args& a, const RowsPlan& p, cudaStream_
   return check_launch("linear_q8");
 }
 
-// What the two kernels were measured to take, in nanoseconds, for products of 17 to 2,048 tokens and the layer sizes
+// How many pairs of blocks run at a time.
+int pair_room() {
+  static int room[kMaxDevices] = {};
+  int& n = room[current_device()];
+  if (n == 0) {
+    auto kernel = q8_pair_kernel<kStoreBf16>;
+    static bool done[kMaxDevices] = {};
+    n = -1;
+    if (reserve(kernel, kPairSmemBytes, done) != kOk) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2048);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kPairSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int v = 0;
+    if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) == cudaSuccess && v > 0) n = v;
+    else cudaGetLastError();
+  }
+  return n > 0 ? n : 0;
+}
+
+// What the three kernels were measured to take, in nanoseconds, for products of 17 to 2,048 tokens and the layer sizes
 // 4,096 / 6,144 / 12,288 / 25,600 and smaller odd ones (rules, right to about a tenth; none knows a size by name).
 // Weight streaming: a cluster's block takes 15 a KB of weight and tokens, and 70 for each token that it finishes; a block
 // with all of K 21 a KB (at least 300 a K block), and 60 a token for its short runs of outputs.
@@ -1008,7 +1236,7 @@ double rows_ns(const RowsPlan& p, int M, int N, int K, bool gated, int bn, int s
 }
 // Tiles: a K block takes 370 / 245 / 205 at 256 / 128 / 64 columns, 540 / 300 / 205 where one tile of tokens reads each
 // weight once, from memory; a tile costs 5,200 / 3,450 / 2,800 beside its K blocks; a cluster's meetings and exchange
-// 2,900 (two blocks) or 4,200.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for
+// 2,900 (two blocks) or 4,200.  Tiles of two SMs (columns = 512): 335 a K block and 5,000 beside.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for
 // 32 bytes of K: 39 against 30 us.)
 struct TilePlan { int columns, splits; double ns; };
 TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
@@ -1029,7 +1257,53 @@ TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
       if (best.ns == 0 || ns < best.ns) best = TilePlan{columns, splits, ns};
     }
   }
+  const int room = n_t > 1 ? pair_room() : 0;
+  if (room > 0) {
+    const int outputs = gated ? 128 : 256;
+    const long long tiles = (n_t + 1) / 2 * ((N + outputs - 1) / outputs), waves = (tiles + room - 1) / room;
+    const double main = n_kb * 335.0 > 2500 || waves == 1 ? n_kb * 335.0 : 2500;
+    const double ns = (double)waves * main + 5000;
+    if (ns < best.ns) best = TilePlan{512, 1, ns};
+  }
   return best;
+}
+
+// A map of y for the epilogue's TMA stores, where its rows allow them (else a valid map that is not used).  (A TMA store
+// clips at whole 16-byte pieces: a row that ends inside one would write beyond it.)
+int output_map(CUtensorMap* my, const CUtensorMap& any, const Args& a, bool f32, int* by_tma) {
+  const int size = f32 ? 4 : 2;
+  *by_tma = (uintptr_t)a.y % 16 == 0 && a.ldy * size % 16 == 0 && (int64_t)a.N * size % 16 == 0;
+  *my = any;
+  if (!*by_tma) return kOk;
+  const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
+  const cuuint64_t stride[1] = {(cuuint64_t)a.ldy * size};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), BM};
+  return encode(my, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, stride, box);
+}
+// A launch of `blocks` blocks in clusters of `cluster` along x (1: none).
+template <typename... KArgs, typename... Given>
+void launch_cluster_x(void (*kernel)(KArgs...), unsigned blocks, int cluster, int smem, cudaStream_t stream, Given&&... given) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (overlap_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kernel, std::forward<Given>(given)...);  // errors are read by check_launch()
 }
 
 template <int MODE, int BF, bool SPLIT>
@@ -1048,42 +1322,14 @@ int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stre
   ta.x_rows = a.M < BM ? (a.M + 7) / 8 * 8 : BM;
   if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, ta.x_rows, kkb)) return rc;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, MODE == kGluBf16 ? BF / 2 : BF, kkb)) return rc;
-  const int size = f32 ? 4 : 2;
-  // (a TMA store clips at whole 16-byte pieces: a row that ends inside one would write beyond it)
-  ta.by_tma = (uintptr_t)a.y % 16 == 0 && a.ldy * size % 16 == 0 && (int64_t)a.N * size % 16 == 0;
-  my = mx;  // not used unless by_tma; a valid map all the same
-  if (ta.by_tma) {
-    const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
-    const cuuint64_t stride[1] = {(cuuint64_t)a.ldy * size};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), BM};
-    if (int rc = encode(&my, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, dims, stride, box)) return rc;
-  }
+  if (int rc = output_map(&my, mx, a, f32, &ta.by_tma)) return rc;
   static bool done[kMaxDevices] = {};
   auto kernel = q8_tile_kernel<MODE, BF, SPLIT>;
   if (int rc = reserve(kernel, C::kSmemBytes, done)) return rc;
   const int sms = sm_count();
   ta.splits = SPLIT ? splits : 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(SPLIT ? (unsigned)(tiles * splits) : (unsigned)(tiles < sms ? tiles : sms));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (SPLIT) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = (unsigned)splits;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (overlap_enabled()) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  cudaLaunchKernelEx(&cfg, kernel, mx, mw, my, a, ta);
+  launch_cluster_x(kernel, SPLIT ? (unsigned)(tiles * splits) : (unsigned)(tiles < sms ? tiles : sms), SPLIT ? splits : 1, C::kSmemBytes, stream,
+                   mx, mw, my, a, ta);
   return check_launch("linear_q8");
 }
 template <int MODE, int BF>
@@ -1092,23 +1338,60 @@ int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stre
 }
 
 template <int MODE>
+int launch_pairs(const Operands& o, const Args& a, cudaStream_t stream) {
+  constexpr int kTileOutputs = MODE == kGluBf16 ? 128 : 256;
+  TileArgs ta = {};
+  ta.n_t_tiles = (a.M + 2 * BM - 1) / (2 * BM);
+  const long long tiles = (long long)ta.n_t_tiles * ((a.N + kTileOutputs - 1) / kTileOutputs);
+  if (tiles > 0x3fffffffLL) return fail(kBadArgument, "linear_q8: too many tiles");
+  ta.n_tiles = (int)tiles;
+  ta.splits = 1;
+  CUtensorMap mx, mw, my;
+  if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, 1)) return rc;
+  if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, BM, 1)) return rc;
+  if (int rc = output_map(&my, mx, a, MODE == kStoreF32 || MODE == kAccumF32, &ta.by_tma)) return rc;
+  static bool done[kMaxDevices] = {};
+  auto kernel = q8_pair_kernel<MODE>;
+  if (int rc = reserve(kernel, kPairSmemBytes, done)) return rc;
+  const long long room = pair_room();
+  launch_cluster_x(kernel, (unsigned)(2 * (tiles < room ? tiles : room)), 2, kPairSmemBytes, stream, mx, mw, my, a, ta);
+  return check_launch("linear_q8");
+}
+
+// The kernel of a product: tiles of p.columns (512: of two SMs; 0: weight streaming by r).
+struct Plan { RowsPlan r; int bn; TilePlan p; };
+Plan plan(int M, int N, int K, bool gated, bool fours) {
+  Plan c;
+  c.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  c.r = plan_rows(N, K, gated, c.bn, fours);
+  c.p = TilePlan{0, 1, 0};
+  if (M <= 16) return c;
+  const int sms = sm_count();
+  const TilePlan tiles = plan_tiles(M, N, K, gated, sms);
+  if (M > 128 || rows_ns(c.r, M, N, K, gated, c.bn, sms) >= tiles.ns) c.p = tiles;
+  return c;
+}
+// the owners of a cluster write four neighbouring outputs of a token at once
+bool in_fours(const void* y, int64_t ldy, int N, int mode) {
+  return N % 4 == 0 && ldy % 4 == 0 && (uintptr_t)y % (mode == kStoreBf16 ? 8 : 16) == 0;
+}
+
+template <int MODE>
 int launch(const Operands& o, const Args& a, cudaStream_t stream) {
   constexpr bool gated = MODE == kGluBf16;
-  const int bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  const int sms = sm_count();
-  // the owners of a cluster write four neighbouring outputs of a token at once
-  const bool fours = a.N % 4 == 0 && a.ldy % 4 == 0 && (uintptr_t)a.y % (MODE == kStoreBf16 ? 8 : 16) == 0;
-  const RowsPlan r = plan_rows(a.N, a.K, gated, bn, fours);
-  if (a.M <= 16) return launch_rows<16, MODE>(o, a, r, stream);
-  const TilePlan p = plan_tiles(a.M, a.N, a.K, gated, sms);
-  if (a.M <= 128 && rows_ns(r, a.M, a.N, a.K, gated, bn, sms) < p.ns) {
-    if (bn == 32) return launch_rows<32, MODE>(o, a, r, stream);
-    if (bn == 64) return launch_rows<64, MODE>(o, a, r, stream);
-    return launch_rows<128, MODE>(o, a, r, stream);
+  const Plan c = plan(a.M, a.N, a.K, gated, in_fours(a.y, a.ldy, a.N, MODE));
+  switch (c.p.columns) {
+    case 512: return launch_pairs<MODE>(o, a, stream);
+    case 256: return launch_tiles<MODE, 256>(o, a, c.p.splits, stream);
+    case 128: return launch_tiles<MODE, 128>(o, a, c.p.splits, stream);
+    case 64: return launch_tiles<gated ? kStoreBf16 : MODE, 64>(o, a, c.p.splits, stream);  // (no gated tile is this narrow)
   }
-  if (p.columns == 256) return launch_tiles<MODE, 256>(o, a, p.splits, stream);
-  if (p.columns == 64) return launch_tiles<gated ? kStoreBf16 : MODE, 64>(o, a, p.splits, stream);  // (no gated tile is this narrow)
-  return launch_tiles<MODE, 128>(o, a, p.splits, stream);
+  switch (c.bn) {
+    case 16: return launch_rows<16, MODE>(o, a, c.r, stream);
+    case 32: return launch_rows<32, MODE>(o, a, c.r, stream);
+    case 64: return launch_rows<64, MODE>(o, a, c.r, stream);
+    default: return launch_rows<128, MODE>(o, a, c.r, stream);
+  }
 }
 }  // namespace
 
@@ -1131,4 +1414,13 @@ extern "C" int skyla_linear_q8(const void* x, int64_t ldx, const float* x_scale,
     case kAccumF32: return launch<kAccumF32>(o, a, stream);
     default: return launch<kGluBf16>(o, a, stream);
   }
+}
+
+// Which kernel takes a product of these sizes whose y is aligned, for tests and measurements: tiles, columns * 16 + splits
+// (512 columns: two SMs a tile); weight streaming, minus the splits (1, 2, 4), or minus 16 times the K blocks of an MMA.
+extern "C" int skyla_linear_q8_plan(int M, int N, int K, int gated) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const Plan c = plan(M, N, K, gated != 0, N % 4 == 0);
+  if (c.p.columns > 0) return c.p.columns * 16 + c.p.splits;
+  return c.r.kstack > 1 ? -16 * c.r.kstack : -c.r.splits;
 }

@@ -113,6 +113,7 @@ def linear_int8(tokens: int, n_out: int, n_in: int, mode: str, copies: int = 0, 
     how = ops.GATED if gated else ops.ACCUMULATE if mode == "accumulate" else ops.STORE
     us = _time(lambda i: ops.linear_q8(x, weights[i], y, how), copies, reps)
     return {"kernel": "linear-int8", "tokens": tokens, "n_out": n_out, "n_in": n_in, "mode": mode, "us": us,
+            "plan": ops.linear_q8_plan(tokens, n_out, n_in, gated),
             "weight_GBps": rows * n_in / us / 1e3, "TOPs": 2.0 * tokens * rows * n_in / us / 1e6}
 
 

@@ -823,6 +823,16 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
     return y
 
 
+def linear_q8_plan(m: int, n_out: int, n_in: int, gated: bool = False) -> str:
+    """Which kernel :func:`linear_q8` gives a product of these sizes (y aligned), in words."""
+    f = _fn("gemm_q8", "skyla_linear_q8_plan", [c_int, c_int, c_int, c_int])
+    code = int(f(m, n_out, n_in, int(gated)))
+    if code > 0:
+        columns, splits = divmod(code, 16)
+        return "tiles of two SMs" if columns == 512 else f"tiles of {columns} columns, K in {splits}"
+    return f"streaming, {-code // 16} K blocks stacked" if code <= -16 else f"streaming, K in {-code}"
+
+
 # ------------------------------------------------------------ attention parts
 def qk_norm_rope_cache(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, nq: int, nkv: int,
                        hd: int, q_norm: Optional[torch.Tensor], k_norm: Optional[torch.Tensor],

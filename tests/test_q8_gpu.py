@@ -217,12 +217,24 @@ def _check_product(m, k, n, x_gap=0, y_gap=0, seed=0):
 
 
 # tokens around every tile, inputs and outputs that no tile divides
-@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 16, 8), (1, 4096, 6144), (2, 130, 77), (8, 4096, 512), (15, 1000, 333),
-                                   (16, 4096, 4096), (17, 4096, 4096), (33, 2048, 1000), (64, 12288, 256), (65, 512, 516),
-                                   (100, 384, 4097), (128, 2560, 2560), (129, 2560, 640), (130, 100, 70), (256, 1024, 96),
-                                   (300, 2561, 1111), (513, 640, 129), (700, 192, 2050)])
+SIZES = [(1, 1, 1), (1, 16, 8), (1, 4096, 6144), (2, 130, 77), (8, 4096, 512), (15, 1000, 333),
+         (16, 4096, 4096), (17, 4096, 4096), (33, 2048, 1000), (64, 12288, 256), (65, 512, 516), (100, 384, 4097),
+         (128, 2560, 2560), (129, 2560, 640), (130, 100, 70), (256, 1024, 96), (300, 2561, 1111), (513, 640, 129),
+         (700, 192, 2050), (20, 2048, 6144), (40, 9728, 2560), (257, 4096, 4000), (1025, 1000, 3001), (2000, 2048, 2048),
+         (2100, 130, 2052), (600, 9728, 2560), (1500, 700, 5000), (27, 1621, 64), (2096, 8863, 215), (20, 11142, 171)]
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
 def test_linear_q8(m, k, n):
     _check_product(m, k, n, seed=m + k + n)
+
+
+def test_every_kernel_is_among_the_sizes():
+    """Weight streaming whole, stacked and in clusters, tiles of every width, whole and split, tiles of two SMs."""
+    plans = {ops.linear_q8_plan(m, n, k, g) for m, k, n in SIZES for g in (False, True)}
+    want = {"streaming, K in 1", "streaming, K in 2", "streaming, K in 4", "tiles of 64 columns, K in 1", "tiles of 64 columns, K in 2",
+            "tiles of 64 columns, K in 4", "tiles of 128 columns, K in 1", "tiles of 128 columns, K in 4", "tiles of two SMs"}
+    assert want <= plans and any("stacked" in p for p in plans), sorted(want - plans)
 
 
 @pytest.mark.parametrize("m,k,n", [(3, 64, 40), (40, 1024, 1024), (200, 256, 300)])
