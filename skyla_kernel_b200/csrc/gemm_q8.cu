@@ -526,26 +526,44 @@ __device__ __forceinline__ void drain(const Args& a, const CUtensorMap* map_y, i
       // a warp takes 32 rows, one after the other, its lanes neighbouring outputs.  (Compact code: a launch starts with
       // cold instruction caches.  Eight rows at a time, pairs of bfloat16 in one store: 333 tokens x 2,561 to 1,111 took
       // 10.4 instead of 8.7 us.)
-#pragma unroll 4
-      for (int i = 0; i < 32; ++i) {
-        const int r = quad * 32 + i;
-        if (tok0 + r >= a.M) break;
-        const int64_t at = (int64_t)(tok0 + r) * a.ldy + f0 + c0;
+      auto at_row = [&](int r, int c) {
+        return out + (uint32_t)r * 128u + (uint32_t)((((c * (f32 ? 4 : 2)) >> 4) ^ (r & 7)) << 4) + (uint32_t)((c * (f32 ? 4 : 2)) & 15);
+      };
+      if (MODE == kAccumF32) {  // eight old values are on their way together
+        const bool live = f0 + c0 + lane < a.N;
+        float* y = (float*)a.y + (int64_t)(tok0 + quad * 32) * a.ldy + f0 + c0 + lane;
+        const int rows = min(32, a.M - tok0 - quad * 32);
+#pragma unroll 1
+        for (int i0 = 0; i0 < rows; i0 += 8) {
+          float o[8];
 #pragma unroll
-        for (int h = 0; h < kCols / 32; ++h) {
-          const int c = lane + 32 * h;
-          const uint32_t from = out + (uint32_t)r * 128u +
-                                (uint32_t)((((c * (f32 ? 4 : 2)) >> 4) ^ (r & 7)) << 4) + (uint32_t)((c * (f32 ? 4 : 2)) & 15);
-          if (f0 + c0 + c >= a.N) continue;
-          if (f32) {
+          for (int i = 0; i < 8; ++i) o[i] = live && i0 + i < rows ? y[(i0 + i) * a.ldy] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
             float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
-            float* y = (float*)a.y + at + c;
-            *y = MODE == kAccumF32 ? __fadd_rn(*y, v) : v;
-          } else {
-            uint16_t v;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-            ((uint16_t*)a.y)[at + c] = v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at_row(quad * 32 + i0 + i, lane)) : "memory");
+            if (live && i0 + i < rows) y[(i0 + i) * a.ldy] = __fadd_rn(o[i], v);
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+          const int r = quad * 32 + i;
+          if (tok0 + r >= a.M) break;
+          const int64_t at = (int64_t)(tok0 + r) * a.ldy + f0 + c0;
+#pragma unroll
+          for (int h = 0; h < kCols / 32; ++h) {
+            const int c = lane + 32 * h;
+            if (f0 + c0 + c >= a.N) continue;
+            if (f32) {
+              float v;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at_row(r, c)) : "memory");
+              ((float*)a.y)[at + c] = v;
+            } else {
+              uint16_t v;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at_row(r, c)) : "memory");
+              ((uint16_t*)a.y)[at + c] = v;
+            }
           }
         }
       }

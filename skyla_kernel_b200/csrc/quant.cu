@@ -2,7 +2,9 @@
 // All three are bound by the memory.  A row belongs to one group of threads (a warp for short rows, else a block), which
 // reads it once, 16 bytes a thread and load, keeps it in registers while the group agrees on the row's largest value
 // (one reduction), and writes its integers.  Elements beyond what the registers hold (kKeep loads a thread) are read again.
-// Rows that do not begin on multiples of 16 bytes, or whose width leaves part of a load, go element by element.
+// Rows that do not begin on multiples of 16 bytes, or whose width leaves part of a load, go by two elements, or one.
+#include <type_traits>
+
 #include "q8.cuh"
 using namespace skyla;
 using namespace skyla::q8;
@@ -10,6 +12,7 @@ SKYLA_EXPORT_ERROR_MESSAGE()
 
 namespace {
 
+template <typename T> struct Type { typedef T type; };
 template <int BYTES> struct Word;
 template <> struct Word<1> { typedef uint8_t type; };
 template <> struct Word<2> { typedef uint16_t type; };
@@ -59,6 +62,7 @@ struct Pack {
 template <int E>
 __device__ __forceinline__ void store_q(int8_t* p, const uint32_t* n) {
   if constexpr (E == 1) *p = (int8_t)n[0];
+  else if constexpr (E == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)__byte_perm(n[0], n[1], 0x0040);
   else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(p) = low_bytes(n);
   else *reinterpret_cast<uint2*>(p) = make_uint2(low_bytes(n), low_bytes(n + 4));
 }
@@ -91,9 +95,10 @@ struct Group {
   }
 };
 
-template <typename T, int E, int kKeep, bool BLOCK>
-__global__ void __launch_bounds__(kKeep == 8 ? 512 : 1024) quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t n_rows, int width, int8_t* __restrict__ q,
-                                int64_t ldq, float* __restrict__ scale) {
+template <typename T, int E, int kKeep, bool BLOCK, bool LONG>
+__global__ void __launch_bounds__(kKeep == 8 ? 512 : 1024) quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t n_rows,
+                                                                           int width, int8_t* __restrict__ q, int64_t ldq,
+                                                                           float* __restrict__ scale) {
   allow_dependents();
   grid_dependency_wait();
   const Group<BLOCK> g;
@@ -101,41 +106,52 @@ __global__ void __launch_bounds__(kKeep == 8 ? 512 : 1024) quantize_kernel(const
   const T* xr = x + g.row * ldx;
   int8_t* qr = q + g.row * ldq;
   const int first = g.rank * E, step = g.size * E;
-  Pack<T, E> kept[kKeep];
+  // kKeep loads of a thread from element e on, all in flight together
+  auto load = [&](int e, Pack<T, E>* p) {
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) p[j].load(xr + e + j * step);
+  };
   unsigned most = 0;
+  auto look = [&](int e, const Pack<T, E>* p) {
 #pragma unroll
-  for (int j = 0; j < kKeep; ++j)
-    if (first + j * step < width) kept[j].load(xr + first + j * step);
-#pragma unroll
-  for (int j = 0; j < kKeep; ++j)
-    if (first + j * step < width) most = kept[j].largest(most);
-  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
-    Pack<T, E> p;
-    p.load(xr + e);
-    most = p.largest(most);
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) most = p[j].largest(most);
+  };
+  Pack<T, E> kept[kKeep];
+  load(first, kept);
+  look(first, kept);
+#pragma unroll 1
+  for (int e = first + kKeep * step; LONG && e < width; e += kKeep * step) {
+    Pack<T, E> more[kKeep];
+    load(e, more);
+    look(e, more);
   }
   g.meet(most, nullptr);
   if (most >= kInfBits) {  // the same for the whole group
-    for (int64_t e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
+    for (int e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
     if (g.rank == 0) scale[g.row] = kNan;
     return;
   }
   const Step s = step_of(most);
-  auto put = [&](int64_t e, const Pack<T, E>& p) {
-    float v[E];
-    uint32_t n[E];
+  auto put = [&](int e, const Pack<T, E>* p) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = p.get(i);
-    round_q<E, sizeof(T) == 2>(v, s, n);
-    store_q<E>(qr + e, n);
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) {
+        float v[E];
+        uint32_t n[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = p[j].get(i);
+        round_q<E, sizeof(T) == 2>(v, s, n);
+        store_q<E>(qr + e + j * step, n);
+      }
   };
-#pragma unroll
-  for (int j = 0; j < kKeep; ++j)
-    if (first + j * step < width) put(first + j * step, kept[j]);
-  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
-    Pack<T, E> p;
-    p.load(xr + e);
-    put(e, p);
+  put(first, kept);
+#pragma unroll 1
+  for (int e = first + kKeep * step; LONG && e < width; e += kKeep * step) {
+    Pack<T, E> more[kKeep];
+    load(e, more);
+    put(e, more);
   }
   if (g.rank == 0) scale[g.row] = s.most / kMost;
 }
@@ -144,7 +160,7 @@ __global__ void __launch_bounds__(kKeep == 8 ? 512 : 1024) quantize_kernel(const
 // With t = x * w the norm is t * inv, inv = 1 / sqrt(mean(x^2) + eps) one number for the row, and 127 t inv / (A inv)
 // = 127 t / A: the integers do not depend on inv, which goes into the scale alone, so the sum of squares and the largest
 // t are found in one pass and one meeting.
-template <typename TX, typename TR, bool ADD, int E, int kKeep, bool BLOCK>
+template <typename TX, typename TR, bool ADD, int E, int kKeep, bool BLOCK, bool LONG>
 __global__ void __launch_bounds__(kKeep == 1 ? 1024 : 512) rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int64_t n_rows,
                                   int width, const float* __restrict__ w, float eps, int8_t* __restrict__ q, int64_t ldq,
                                   float* __restrict__ scale) {
@@ -158,58 +174,51 @@ __global__ void __launch_bounds__(kKeep == 1 ? 1024 : 512) rmsnorm_q8_kernel(TX*
   const int first = g.rank * E, step = g.size * E;
   float ss = 0.f;
   unsigned most = 0;
-  // t of E elements, the sum written back
-  auto take = [&](int64_t e, Pack<TX, E>& p, const Pack<TR, E>& add, const Pack<float, E>& weight, float* t) {
-    if (ADD) {
+  // kKeep loads of a thread from element e on, all in flight together: the sums written back, and their t
+  auto take = [&](int e, float (*t)[E]) {
+    Pack<TX, E> p[kKeep];
+    Pack<TR, E> add[ADD ? kKeep : 1];
 #pragma unroll
-      for (int i = 0; i < E; ++i) p.set(i, p.get(i) + add.get(i));
-      p.store(xr + e);
-    }
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) {
+        p[j].load(xr + e + j * step);
+        if (ADD) add[j].load(rr + e + j * step);
+      }
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float v = p.get(i);
-      ss = fmaf(v, v, ss);
-      t[i] = v * weight.get(i);
-      most = max(most, abs_bits(t[i]));
-    }
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) {
+        Pack<float, E> weight;
+        weight.load(w + e + j * step);
+        if (ADD) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) p[j].set(i, p[j].get(i) + add[ADD ? j : 0].get(i));
+          p[j].store(xr + e + j * step);
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float v = p[j].get(i);
+          ss = fmaf(v, v, ss);
+          t[j][i] = v * weight.get(i);
+          most = max(most, abs_bits(t[j][i]));
+        }
+      }
   };
   float kept[kKeep][E];
-  {
-    Pack<TX, E> p[kKeep];
-    Pack<TR, E> add[kKeep];
-#pragma unroll
-    for (int j = 0; j < kKeep; ++j)
-      if (first + j * step < width) {
-        p[j].load(xr + first + j * step);
-        if (ADD) add[j].load(rr + first + j * step);
-      }
-#pragma unroll
-    for (int j = 0; j < kKeep; ++j)
-      if (first + j * step < width) {
-        Pack<float, E> weight;
-        weight.load(w + first + j * step);
-        take(first + j * step, p[j], add[j], weight, kept[j]);
-      }
-  }
-  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {
-    Pack<TX, E> p;
-    Pack<TR, E> add;
-    Pack<float, E> weight;
-    p.load(xr + e);
-    if (ADD) add.load(rr + e);
-    weight.load(w + e);
-    float t[E];
-    take(e, p, add, weight, t);
+  take(first, kept);
+#pragma unroll 1
+  for (int e = first + kKeep * step; LONG && e < width; e += kKeep * step) {
+    float more[kKeep][E];
+    take(e, more);
   }
   g.meet(most, &ss);
   // the same for the whole group (the mean square and eps may both be zero; the scale is one thread's work)
   if (most >= kInfBits || abs_bits(ss) >= kInfBits || (eps == 0.f && ss / (float)width == 0.f)) {
-    for (int64_t e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
+    for (int e = first; e < width; e += step) store_q<E>(qr + e, kZeros);
     if (g.rank == 0) scale[g.row] = kNan;
     return;
   }
   const Step s = step_of(most);
-  auto put = [&](int64_t e, const float* t) {
+  auto put = [&](int e, const float* t) {
     uint32_t n[E];
     round_q<E, false>(t, s, n);
     store_q<E>(qr + e, n);
@@ -217,15 +226,22 @@ __global__ void __launch_bounds__(kKeep == 1 ? 1024 : 512) rmsnorm_q8_kernel(TX*
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
     if (first + j * step < width) put(first + j * step, kept[j]);
-  for (int64_t e = first + (int64_t)kKeep * step; e < width; e += step) {  // (this thread wrote these sums itself)
-    Pack<TX, E> p;
-    Pack<float, E> weight;
-    p.load(xr + e);
-    weight.load(w + e);
-    float t[E];
+#pragma unroll 1
+  for (int e = first + kKeep * step; LONG && e < width; e += kKeep * step) {  // (this thread wrote these sums itself)
+    Pack<TX, E> p[kKeep];
 #pragma unroll
-    for (int i = 0; i < E; ++i) t[i] = p.get(i) * weight.get(i);
-    put(e, t);
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) p[j].load(xr + e + j * step);
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (e + j * step < width) {
+        Pack<float, E> weight;
+        weight.load(w + e + j * step);
+        float t[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) t[i] = p[j].get(i) * weight.get(i);
+        put(e + j * step, t);
+      }
   }
   if (g.rank == 0) scale[g.row] = s.most * (1.0f / sqrtf(ss / (float)width + eps)) / kMost;
 }
@@ -272,18 +288,18 @@ bool rows_on(const void* p, int64_t ld, int size, int bytes) { return (uintptr_t
 // does once for its row, some 200 instructions, counts for that many, and more registers a thread cost more than that gives
 // (8,192 x 4,096 with its residual: 74 / 59 / 80 us at two / four / eight loads).  Only the quantisation of long rows
 // (`most_kept` 8), whose loads stay as they come, gains by eight (2,048 x 12,288 of 32 bits: 35 to 28 us).
-struct Shape { int threads; int keep; bool block; };
+struct Shape { int threads; int keep; bool block; bool longer; };
 Shape shape_for(int64_t n_rows, int width, int E, int most_kept) {
   const int64_t loads = ((int64_t)width + E - 1) / E;
   // a warp a row, eight rows a block
-  if (loads <= 32 * 4 && n_rows >= 8) return {256, loads <= 32 ? 1 : 4, false};
+  if (loads <= 32 * 4 && n_rows >= 8) return {256, loads <= 32 ? 1 : 4, false, false};
   // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last
   int64_t threads = n_rows < 592 && loads <= 1024 ? loads : (loads + 3) / 4;
   if (n_rows < 592 && loads > 1024) threads = 512;
   if (n_rows >= 592 && threads > 512) threads = (loads + most_kept - 1) / most_kept;
   if (threads > 512 && loads > 1024) threads = 512;
   threads = threads < 64 ? 64 : (threads + 31) / 32 * 32;
-  return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : most_kept, true};
+  return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : most_kept, true, loads > most_kept * threads};
 }
 dim3 grid_for(int64_t n_rows, const Shape& s) { return dim3((unsigned)(s.block ? n_rows : (n_rows + s.threads / 32 - 1) / (s.threads / 32))); }
 
@@ -293,8 +309,9 @@ void launch_quantize(const Shape& s, const void* x, int64_t ldx, int64_t n_rows,
   auto go = [&](auto kernel) {
     launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const T*)x, ldx, n_rows, width, (int8_t*)q, ldq, scale);
   };
-  if (s.block) s.keep == 1 ? go(quantize_kernel<T, E, 1, true>) : s.keep == 4 ? go(quantize_kernel<T, E, 4, true>) : go(quantize_kernel<T, E, 8, true>);
-  else s.keep == 1 ? go(quantize_kernel<T, E, 1, false>) : go(quantize_kernel<T, E, 4, false>);
+  if (!s.block) s.keep == 1 ? go(quantize_kernel<T, E, 1, false, false>) : go(quantize_kernel<T, E, 4, false, false>);
+  else if (s.longer) go(quantize_kernel<T, E, 8, true, true>);
+  else s.keep == 1 ? go(quantize_kernel<T, E, 1, true, false>) : s.keep == 4 ? go(quantize_kernel<T, E, 4, true, false>) : go(quantize_kernel<T, E, 8, true, false>);
 }
 template <typename TX, typename TR, bool ADD, int E>
 void launch_norm(const Shape& s, void* x, int64_t ldx, const void* residual, int64_t ldr, int64_t n_rows, int width, const float* w,
@@ -303,8 +320,9 @@ void launch_norm(const Shape& s, void* x, int64_t ldx, const void* residual, int
     launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (TX*)x, ldx, (const TR*)residual, ldr, n_rows, width,
                       w, eps, (int8_t*)q, ldq, scale);
   };
-  if (s.block) s.keep == 1 ? go(rmsnorm_q8_kernel<TX, TR, ADD, E, 1, true>) : go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, true>);
-  else s.keep == 1 ? go(rmsnorm_q8_kernel<TX, TR, ADD, E, 1, false>) : go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, false>);
+  if (!s.block) s.keep == 1 ? go(rmsnorm_q8_kernel<TX, TR, ADD, E, 1, false, false>) : go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, false, false>);
+  else if (s.longer) go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, true, true>);
+  else s.keep == 1 ? go(rmsnorm_q8_kernel<TX, TR, ADD, E, 1, true, false>) : go(rmsnorm_q8_kernel<TX, TR, ADD, E, 4, true, false>);
 }
 }  // namespace
 
@@ -316,6 +334,8 @@ extern "C" int skyla_quantize_rows(const void* x, int x_dtype, int64_t ldx, int6
     constexpr int E = 16 / sizeof(T);
     if (width % E == 0 && rows_on(x, ldx, sizeof(T), 16) && rows_on(q, ldq, 1, E))
       launch_quantize<T, E>(shape_for(n_rows, width, E, 8), x, ldx, n_rows, width, q, ldq, scale, stream);
+    else if (width % 2 == 0 && rows_on(x, ldx, sizeof(T), 2 * sizeof(T)) && rows_on(q, ldq, 1, 2))
+      launch_quantize<T, 2>(shape_for(n_rows, width, 2, 8), x, ldx, n_rows, width, q, ldq, scale, stream);
     else
       launch_quantize<T, 1>(shape_for(n_rows, width, 1, 8), x, ldx, n_rows, width, q, ldq, scale, stream);
   });
@@ -329,20 +349,27 @@ extern "C" int skyla_rmsnorm_q8(void* x, int x_dtype, int64_t ldx, const void* r
   if (int rc = check_sizes("rmsnorm_q8", n_rows, width, ldx, ldq)) return rc;
   if (!(eps >= 0.f)) return fail(kBadArgument, "rmsnorm_q8: eps must not be negative");
   SKYLA_DISPATCH(x_dtype, TX, {
-    constexpr int E = 16 / sizeof(TX);
-    const int r_size = r_dtype == kF32 ? 4 : 2;
-    // (an element of a residual of another type than x's takes E * r_size bytes a load: 8, 16 or twice 16)
-    const bool vec = width % E == 0 && rows_on(x, ldx, sizeof(TX), 16) && rows_on(q, ldq, 1, E) && (uintptr_t)weight % 16 == 0 &&
-                     (residual == nullptr || rows_on(residual, ldr, r_size, E * r_size < 16 ? E * r_size : 16));
-    if (residual == nullptr) {
-      if (vec) launch_norm<TX, float, false, E>(shape_for(n_rows, width, E, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
-      else launch_norm<TX, float, false, 1>(shape_for(n_rows, width, 1, 4), x, ldx, nullptr, 0, n_rows, width, weight, eps, q, ldq, scale, stream);
-    } else {
-      SKYLA_DISPATCH(r_dtype, TR, {
-        if (vec) launch_norm<TX, TR, true, E>(shape_for(n_rows, width, E, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
-        else launch_norm<TX, TR, true, 1>(shape_for(n_rows, width, 1, 4), x, ldx, residual, ldr, n_rows, width, weight, eps, q, ldq, scale, stream);
-      });
-    }
+    // whether rows can go by e elements: x, residual, weight and q begin on as many whole ones (a load takes at most 16 bytes)
+    auto on = [&](int e) {
+      const int r_bytes = e * (r_dtype == kF32 ? 4 : 2), w_bytes = 4 * e;
+      return width % e == 0 && rows_on(x, ldx, sizeof(TX), e * (int)sizeof(TX)) && rows_on(q, ldq, 1, e) &&
+             (uintptr_t)weight % (w_bytes < 16 ? w_bytes : 16) == 0 &&
+             (residual == nullptr || rows_on(residual, ldr, r_dtype == kF32 ? 4 : 2, r_bytes < 16 ? r_bytes : 16));
+    };
+    auto by = [&](auto e, auto tr, auto add) {
+      constexpr int E = decltype(e)::value;
+      launch_norm<TX, typename decltype(tr)::type, decltype(add)::value, E>(shape_for(n_rows, width, E, 4), x, ldx, residual, ldr, n_rows,
+                                                                           width, weight, eps, q, ldq, scale, stream);
+    };
+    auto with = [&](auto tr, auto add) {
+      // (four elements of a bfloat16 row with a 32-bit residual, for the registers' sake)
+      constexpr int E = 16 / (decltype(add)::value && sizeof(typename decltype(tr)::type) > sizeof(TX) ? 4 : sizeof(TX));
+      if (on(E)) by(std::integral_constant<int, E>(), tr, add);
+      else if (on(2)) by(std::integral_constant<int, 2>(), tr, add);
+      else by(std::integral_constant<int, 1>(), tr, add);
+    };
+    if (residual == nullptr) with(Type<float>(), std::false_type());
+    else SKYLA_DISPATCH(r_dtype, TR, { with(Type<TR>(), std::true_type()); });
   });
   return check_launch("rmsnorm_q8");
 }
@@ -356,8 +383,10 @@ extern "C" int skyla_dequantize_rows(const void* q, int64_t ldq, const float* sc
       launch_overlapped(kernel, grid_for(n_rows, s), dim3(s.threads), 0, stream, (const int8_t*)q, ldq, scale, n_rows, width, (T*)out, ldo);
     };
     const bool vec = width % 8 == 0 && rows_on(q, ldq, 1, 8) && rows_on(out, ldo, sizeof(T), 16);
-    const Shape s = shape_for(n_rows, width, vec ? 8 : 1, 4);
+    const bool two = !vec && width % 2 == 0 && rows_on(q, ldq, 1, 2) && rows_on(out, ldo, sizeof(T), 2 * sizeof(T));
+    const Shape s = shape_for(n_rows, width, vec ? 8 : two ? 2 : 1, 4);
     if (vec) s.block ? go(dequantize_kernel<T, 8, true>, s) : go(dequantize_kernel<T, 8, false>, s);
+    else if (two) s.block ? go(dequantize_kernel<T, 2, true>, s) : go(dequantize_kernel<T, 2, false>, s);
     else s.block ? go(dequantize_kernel<T, 1, true>, s) : go(dequantize_kernel<T, 1, false>, s);
   });
   return check_launch("dequantize_rows");
