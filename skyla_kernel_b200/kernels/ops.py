@@ -250,7 +250,7 @@ def default_state(device) -> KernelState:
 
 
 def _state(state: Optional[KernelState], t: torch.Tensor) -> KernelState:
-    return state if state is not None else _DEFAULT_STATES.get(t.device) or default_state(t.device)
+    return state if state is not None else default_state(t.device)
 
 
 def check_device_errors(device) -> None:
@@ -611,6 +611,13 @@ def q8_rows(n: int, width: int, device) -> Q8Rows:
 _MOST = 1 << 29  # rows or elements of a row: the launchers count them in 32 bits
 
 
+def _room(x: torch.Tensor, n: int, width: int):
+    """:func:`q8_rows` on the device of ``x`` (q, scale, row stride): room for its rows."""
+    ld = -(-width // 16) * 16
+    q = x.new_empty((n, ld), dtype=torch.int8)
+    return q if ld == width else q[:, :width], x.new_empty(n, dtype=torch.float32), ld
+
+
 def _dims(t: torch.Tensor, what: str):
     """(rows, width, row stride) of a 2-D tensor whose rows are contiguous."""
     if t.dim() != 2:
@@ -643,16 +650,31 @@ def _q8_dims(rows: Q8Rows, what: str, dims=_dims):
     return n, width, ld
 
 
-def _device_of(*tensors) -> int:
+def _device_of(first: torch.Tensor, *others) -> int:
     """The one CUDA device of the operands."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        at = t.get_device()
-        if at < 0 or not t.is_cuda:
-            raise KernelError("kernel operands must be CUDA tensors; there is no host path")
-        if at != dev:
-            raise KernelError(f"kernel operands on devices {dev} and {at}")
+    if not first.is_cuda:
+        raise KernelError("kernel operands must be CUDA tensors; there is no host path")
+    dev = first.get_device()
+    for t in others:
+        if t.get_device() != dev or not t.is_cuda:
+            raise KernelError(f"kernel operands on {first.device} and {t.device}")
     return dev
+
+
+_FLAGS = {}
+
+
+def _default_flag(dev: int) -> torch.Tensor:
+    """The error word of a device's default state."""
+    flag = _FLAGS.get(dev)
+    if flag is None:
+        flag = _FLAGS[dev] = default_state(torch.device("cuda", dev)).error_flag
+    return flag
+
+
+# (what torch.cuda.current_device() and current_stream() ask; operands on a device have initialised CUDA before)
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+_get_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 class _Launcher:
@@ -668,11 +690,11 @@ class _Launcher:
         f = self.f
         if f is None:
             f = self.f = _fn(self.module, self.name, self.argtypes)
-        if dev == torch._C._cuda_getDevice():
-            _check(self.module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+        if dev == _get_device():
+            _check(self.module, f(*args, _get_stream(dev)))
         else:
             with torch.cuda.device(dev):
-                _check(self.module, f(*args, torch._C._cuda_getCurrentRawStream(dev)))
+                _check(self.module, f(*args, _get_stream(dev)))
 
 
 _quantize_rows = _Launcher("quant", "skyla_quantize_rows", c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p)
@@ -693,12 +715,16 @@ def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
     n, width, ld = _dims(x, "quantize_rows")
     code = dtype_code(x)
     if out is None:
-        out = q8_rows(n, width, x.device)
-    q, scale = out
-    m, w, ldq = _q8_dims(out, "quantize_rows", _written_dims)
-    if m != n or w != width:
-        raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
-    _quantize_rows(_device_of(x, q, scale), x.data_ptr(), code, ld, n, width, q.data_ptr(), ldq, scale.data_ptr())
+        dev = _device_of(x)
+        q, scale, ldq = _room(x, n, width)
+        out = Q8Rows(q, scale)
+    else:
+        q, scale = out
+        m, w, ldq = _q8_dims(out, "quantize_rows", _written_dims)
+        if m != n or w != width:
+            raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
+        dev = _device_of(x, q, scale)
+    _quantize_rows(dev, x.data_ptr(), code, ld, n, width, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
 
@@ -727,21 +753,24 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         raise KernelError(f"rmsnorm_q8: the weight must be a contiguous float32 vector of {width}")
     if not eps >= 0:
         raise KernelError(f"rmsnorm_q8: eps must not be negative, got {eps}")
-    if out is None:
-        out = q8_rows(n, width, x.device)
-    q, scale = out
-    m, w, ldq = _q8_dims(out, "rmsnorm_q8", _written_dims)
-    if m != n or w != width:
-        raise KernelError(f"rmsnorm_q8: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
     if residual is None:
         r_ptr, r_code, ldr = None, 0, 0
-        dev = _device_of(x, weight, q, scale)
+        dev = _device_of(x, weight)
     else:
         m, w, ldr = _dims(residual, "rmsnorm_q8")
         if m != n or w != width:
             raise KernelError(f"rmsnorm_q8: residual {tuple(residual.shape)} against x {tuple(x.shape)}")
         r_ptr, r_code = residual.data_ptr(), dtype_code(residual)
-        dev = _device_of(x, weight, q, scale, residual)
+        dev = _device_of(x, weight, residual)
+    if out is None:
+        q, scale, ldq = _room(x, n, width)
+        out = Q8Rows(q, scale)
+    else:
+        q, scale = out
+        m, w, ldq = _q8_dims(out, "rmsnorm_q8", _written_dims)
+        if m != n or w != width:
+            raise KernelError(f"rmsnorm_q8: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
+        _device_of(x, q, scale)
     _rmsnorm_q8(dev, x.data_ptr(), code, ld, r_ptr, r_code, ldr, n, width, weight.data_ptr(), eps, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
@@ -809,8 +838,12 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
     if code != (F32 if mode == ACCUMULATE else BF16 if mode == GATED else code):
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
-    flag = _state(state, y).error_flag if y.is_cuda else y
-    dev = _device_of(q, scale, rows.q, rows.scale, y, flag)
+    dev = _device_of(q, scale, rows.q, rows.scale, y)
+    if state is None:
+        flag = _default_flag(dev)
+    else:
+        flag = state.error_flag
+        _device_of(y, flag)
     if m == 1:
         ldx = w.ld  # the distance to a next row that is not there
     if ldx % 16 == 0 and ldx >= k and q.data_ptr() % 16 == 0:
