@@ -3,11 +3,13 @@
 //   acc[t, f] = sum_k x[t, k] W[f, k]   tcgen05.mma kind::i8, 32-bit integers in TMEM: exact in every order, so
 //                                       how a product is cut never shows in its result
 //   v = acc * x_scale[t] * w_scale[f]   y = v, y += v, or y = silu(v of the gate) * v of the up
-// Two kernels, as for bfloat16 (gemm_tc.cu, gemm_prompt.cu); a K block is 128 bytes, one swizzle row, here 128
-// elements, and an instruction takes 32 of them:
-//   up to 128 tokens  the weight streams through every SM once; the weight's rows are the MMA's 128 rows and the
-//                     tokens its columns;
-//   more              the tokens are the MMA's rows, so that a thread of the epilogue owns a token's row.
+// Three kernels; a K block is 128 bytes, one swizzle row, here 128 elements, and an instruction takes 32 of them:
+//   q8_rows_kernel   few tokens: the weight streams through every SM once; the weight's rows are the MMA's 128 rows
+//                    and the tokens its columns;
+//   q8_tile_kernel   tiles of 128 tokens: the tokens are the MMA's rows, so that a thread of the epilogue owns a
+//                    token's row;
+//   q8_pair_kernel   tiles of 256 tokens on two SMs, where there are many.
+// plan() chooses by what they were measured to take.
 // Every mbarrier wait is bounded: on a timeout the block records an error code (1 to 19), lets the loads it issued
 // land, frees its TMEM and returns.
 #include <cuda.h>
@@ -47,6 +49,18 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a, uint64_t b,
 // D 32-bit integers, A and B signed 8-bit, both K-major, N columns, M = 128
 __device__ __forceinline__ uint32_t idesc_i8(int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+// The 128 threads of the epilogue meet and agree: whether all of them say so.  (A wait that gave up in one warp and
+// not in another must not leave the others at a barrier.)
+__device__ __forceinline__ bool all_agree(bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"((uint32_t)mine) : "memory");
+  return r != 0;
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -746,8 +760,7 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (!waited) grid_dependency_wait();
       waited = true;
       const float xs = tok < a.M ? a.x_scale[tok] : 0.f;
-      asm volatile("barrier.sync 1, 128;" ::: "memory");
-      bool ok = mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3);
+      const bool ok = all_agree(mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3));
       if (!SPLIT && !ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_base + buf * BF + ((uint32_t)(quad * 32) << 16);
@@ -987,8 +1000,7 @@ q8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (!waited) grid_dependency_wait();
       waited = true;
       const float xs = tok < a.M ? a.x_scale[tok] : 0.f;
-      asm volatile("barrier.sync 1, 128;" ::: "memory");
-      if (!mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3)) break;
+      if (!all_agree(mbar_wait(acc_full_bar(buf), (it >> 1) & 1, &abort_flag, a.error_flag, 3))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_base + buf * BF + ((uint32_t)(quad * 32) << 16);
       if (tok0 < a.M)  // the same for the block
@@ -1239,7 +1251,7 @@ int pair_room() {
 }
 
 // What the three kernels were measured to take, in nanoseconds, for products of 17 to 2,048 tokens and the layer sizes
-// 4,096 / 6,144 / 12,288 / 25,600 and smaller odd ones (rules, right to about a tenth; none knows a size by name).
+// 4,096 / 6,144 / 12,288 / 25,600 and smaller odd ones (right to about a tenth).
 // Weight streaming: a cluster's block takes 15 a KB of weight and tokens, and 70 for each token that it finishes; a block
 // with all of K 21 a KB (at least 300 a K block), and 60 a token for its short runs of outputs.
 double rows_ns(const RowsPlan& p, int M, int N, int K, bool gated, int bn, int sms) {
