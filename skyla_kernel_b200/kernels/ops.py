@@ -798,6 +798,7 @@ class Q8Weight:
             kept.copy_(q)
             q, ld = kept, _dims(kept, "Q8Weight")[2]
         if q.is_cuda:
+            _default_flag(q.get_device())  # here, so that a product's first call may lie inside a capture
             torch.cuda.synchronize(q.device)
         self.rows, self.gated, self.n_in, self.ld = Q8Rows(q, scale), bool(gated), width, ld
         self.n_out = n // 2 if gated else n

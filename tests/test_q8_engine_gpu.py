@@ -108,6 +108,15 @@ def test_generation_through_the_entry_point(folders):
         assert float(gap.max()) <= 2 * WORST * float(logits.abs().max())
 
 
+def test_the_command_line(folders, capsys):
+    from skyla_kernel_b200.cli import main
+    assert main(["run", folders["B"], "--prompt-ids", "1,2,3,4", "--prompt-ids", "7", "-n", "5", "--stop-id", "-1", "--weights", "int8"]) == 0
+    lines = capsys.readouterr().out.strip().splitlines()
+    assert [len(line.split()) for line in lines] == [5, 5]
+    with pytest.raises(ValueError):
+        main(["run", folders["B"], "--prompt-ids", "1", "--dtype", "float32", "--weights", "int8"])
+
+
 def test_weights_take_half_the_memory(folders):
     from skyla_kernel_b200.engine import Engine
     bf16 = Engine.from_folder(folders["D"])

@@ -1,5 +1,6 @@
 """The 8-bit operators against their definitions in 64 bits."""
 import math
+import os
 
 import pytest
 import torch
@@ -8,6 +9,7 @@ from skyla_kernel_b200.kernels import ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF16, F32 = torch.bfloat16, torch.float32
 FLOOR = 127 * 2.0 ** -126  # under a row's largest magnitude
 
@@ -320,6 +322,32 @@ def test_a_weight_is_not_laid_out_inside_a_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(rows.q, _want(w)[0])
+
+
+def test_a_product_whose_first_call_is_captured():
+    """In a process of its own: nothing of the package has run before."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from skyla_kernel_b200.kernels import ops
+w = ops.Q8Weight.quantize(torch.ones(64, 128, device="cuda"))
+x = ops.quantize_rows(torch.ones(200, 128, device="cuda"))
+y = torch.zeros(200, 64, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.linear_q8(x, w, y, ops.ACCUMULATE)
+ops.check_device_errors("cuda:0")
+assert not y.any()
+for _ in range(3):
+    graph.replay()
+ops.check_device_errors("cuda:0")
+v = torch.full((200, 64), float(128 * 127 * 127), device="cuda") * x.scale[:, None] * w.rows.scale
+assert torch.equal(y, v + v + v), (y, v)
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_a_weight_of_the_first_outputs():
