@@ -286,18 +286,22 @@ bool rows_on(const void* p, int64_t ld, int size, int bytes) { return (uintptr_t
 
 // How a row is shared out: threads, and loads that each keeps.  Four loads a thread where there are many rows: what a thread
 // does once for its row, some 200 instructions, counts for that many, and more registers a thread cost more than that gives
-// (8,192 x 4,096 with its residual: 74 / 59 / 80 us at two / four / eight loads).  Only the quantisation of long rows
-// (`most_kept` 8), whose loads stay as they come, gains by eight (2,048 x 12,288 of 32 bits: 35 to 28 us).
+// (norm of 8,192 x 4,096 with its residual: 74 / 59 / 80 us at two / four / eight loads).  The quantisation (`most_kept` 8),
+// whose loads stay as they come, gains by eight for long rows and for many of bfloat16 (2,048 x 12,288: 20.7 to 17.1 us of
+// bfloat16, 35 to 27 of 32 bits; 24,576 x 4,096 of bfloat16: 58.3 to 53.6; but 2,048 x 4,096: 7.3 to 8.4).
 struct Shape { int threads; int keep; bool block; bool longer; };
 Shape shape_for(int64_t n_rows, int width, int E, int most_kept) {
   const int64_t loads = ((int64_t)width + E - 1) / E;
   // a warp a row, eight rows a block
   if (loads <= 32 * 4 && n_rows >= 8) return {256, loads <= 32 ? 1 : 4, false, false};
-  // few rows: as many threads as the row has loads, for the shortest way from its first byte to its last
-  int64_t threads = n_rows < 592 && loads <= 1024 ? loads : (loads + 3) / 4;
-  if (n_rows < 592 && loads > 1024) threads = 512;
-  if (n_rows >= 592 && threads > 512) threads = (loads + most_kept - 1) / most_kept;
-  if (threads > 512 && loads > 1024) threads = 512;
+  int64_t threads;
+  if (n_rows < 592) {  // few rows: as many threads as loads, for the shortest way from the row's first byte to its last
+    threads = loads <= 1024 ? loads : 512;
+  } else {
+    const bool eight = loads > 2048 || (E == 8 && (loads >= 1024 || n_rows >= 8192));
+    threads = (loads + (eight ? most_kept : 4) - 1) / (eight ? most_kept : 4);
+    if (threads > 512) threads = 512;
+  }
   threads = threads < 64 ? 64 : (threads + 31) / 32 * 32;
   return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : most_kept, true, loads > most_kept * threads};
 }
