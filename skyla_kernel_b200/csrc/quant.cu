@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kKeep == 8 ? 512 : 1024) quantize_kernel(const
 // = 127 t / A: the integers do not depend on inv, which goes into the scale alone, so the sum of squares and the largest
 // t are found in one pass and one meeting.
 template <typename TX, typename TR, bool ADD, int E, int kKeep, bool BLOCK, bool LONG>
-__global__ void __launch_bounds__(kKeep == 1 ? 1024 : 512) rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int64_t n_rows,
+__global__ void __launch_bounds__(kKeep == 1 ? 1024 : 768) rmsnorm_q8_kernel(TX* __restrict__ x, int64_t ldx, const TR* __restrict__ residual, int64_t ldr, int64_t n_rows,
                                   int width, const float* __restrict__ w, float eps, int8_t* __restrict__ q, int64_t ldq,
                                   float* __restrict__ scale) {
   allow_dependents();
@@ -300,7 +300,7 @@ Shape shape_for(int64_t n_rows, int width, int E, int most_kept) {
   } else {
     const bool eight = loads > 2048 || (E == 8 && (loads >= 1024 || n_rows >= 8192));
     threads = (loads + (eight ? most_kept : 4) - 1) / (eight ? most_kept : 4);
-    if (threads > 512) threads = 512;
+    if (threads > 512) threads = most_kept == 4 && loads <= 4 * 768 ? 768 : 512;
   }
   threads = threads < 64 ? 64 : (threads + 31) / 32 * 32;
   return {(int)threads, loads <= threads ? 1 : loads <= 4 * threads ? 4 : most_kept, true, loads > most_kept * threads};
