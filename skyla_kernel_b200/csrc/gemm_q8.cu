@@ -439,8 +439,8 @@ q8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // tokens at a time are laid out in one of two 16 KB buffers and leave by a TMA store (or reduce-add: y += v never reads
 // y), or, where y's rows do not allow that, row by row in order.
 // SPLIT: few tiles; the blocks of a cluster share one tile, each with a run of its K blocks.  They leave their
-// accumulators in shared memory (the ring, idle by then), and each finishes an equal part of the columns from all of
-// them, read through distributed shared memory: whole numbers, so the result does not show the cut.
+// accumulators in shared memory (the ring, idle by then), and each finishes an equal part of the outputs, or of the
+// tokens, from all of them: whole numbers, so the result does not show the cut.
 constexpr int kOutBytes = BM * 128;  // 128 tokens x 128 bytes
 constexpr int kMaxSplits = 4;
 
@@ -604,6 +604,86 @@ struct TileArgs {
   int splits;         // blocks of a cluster (SPLIT), each with an equal run of the K blocks; else 1
 };
 
+// Sixteen columns of a token, summed over the accumulators of a cluster's blocks through distributed shared memory (`mine`:
+// where the token's lie in each); the loads of all blocks are in flight together.
+__device__ __forceinline__ void split_sum16(uint32_t mine, int splits, int c0, uint32_t* r) {
+  uint32_t v[kMaxSplits][16];
+#pragma unroll
+  for (int q = 0; q < kMaxSplits; ++q) {
+    if (q >= splits) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[q][j] = 0;
+      continue;
+    }
+    uint32_t from;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(mine + (uint32_t)(c0 / 4) * (BM * 16u)), "r"((uint32_t)q));
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[q][4 * c]), "=r"(v[q][4 * c + 1]),
+                   "=r"(v[q][4 * c + 2]), "=r"(v[q][4 * c + 3]) : "r"(from + (uint32_t)c * (BM * 16u)) : "memory");
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) r[j] = v[0][j] + v[1][j] + v[2][j] + v[3][j];
+}
+
+// The end of a tile of 64 outputs that four blocks share: each finishes 32 of the tokens, a thread sixteen outputs of one,
+// written straight away.  (The blocks taking turns at the columns through drain(), two of the four have nothing to do: 500
+// tokens x 16,384 to 512 took 13.0 instead of 11.6 us.  With more outputs a thread, drain()'s order of writing wins: two
+// splits of 4,096 to 4,096 at 128 tokens 8.7 against 9.8.)
+template <int MODE, int BF>
+__device__ __forceinline__ void finish_tokens(const Args& a, const TileArgs& ta, const float* ws, uint32_t ring, int f0, int tok0, int rank,
+                                              int et) {
+  constexpr bool f32 = MODE == kStoreF32 || MODE == kAccumF32;
+  const int row = rank * 32 + et % 32, c0 = et / 32 * 16, tok = tok0 + row;
+  const int f = f0 + c0, n = min(16, a.N - f);
+  if (tok >= a.M || n <= 0) return;
+  const float xs = a.x_scale[tok];
+  const uint32_t mine = ring + 16u * (uint32_t)row;
+  const bool whole = ta.by_tma && n == 16;  // as vectors: y's rows begin and end on 16 bytes
+  float* y32 = (float*)a.y + (int64_t)tok * a.ldy + f;
+  __nv_bfloat16* y16 = (__nv_bfloat16*)a.y + (int64_t)tok * a.ldy + f;
+  float old[16];
+  if (MODE == kAccumF32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 o = whole ? reinterpret_cast<const float4*>(y32)[j]
+                             : make_float4(4 * j < n ? y32[4 * j] : 0.f, 4 * j + 1 < n ? y32[4 * j + 1] : 0.f,
+                                           4 * j + 2 < n ? y32[4 * j + 2] : 0.f, 4 * j + 3 < n ? y32[4 * j + 3] : 0.f);
+      old[4 * j] = o.x; old[4 * j + 1] = o.y; old[4 * j + 2] = o.z; old[4 * j + 3] = o.w;
+    }
+  }
+  uint32_t r[16];
+  float v[16];
+  split_sum16(mine, 4, c0, r);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = scaled((int)r[j], xs, ws[c0 + j]);
+  if (MODE == kGluBf16) {
+    split_sum16(mine, 4, BF / 2 + c0, r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = silu_times(v[j], scaled((int)r[j], xs, ws[BF / 2 + c0 + j]));
+  }
+  if (MODE == kAccumF32) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __fadd_rn(old[j], v[j]);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) {
+        if (f32) y32[j] = v[j];
+        else y16[j] = __float2bfloat16_rn(v[j]);
+      }
+  } else if (f32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(y32)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      reinterpret_cast<uint4*>(y16)[j] = make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
+                                                    pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+  }
+}
+
 template <int MODE, int BF, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -764,10 +844,10 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (!SPLIT && !ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_base + buf * BF + ((uint32_t)(quad * 32) << 16);
-      // the ring as a split leaves its accumulator there: [piece of four columns][row], a warp's rows 512 bytes in a row
-      const uint32_t left = base + 16u * (uint32_t)row;
-      if (SPLIT) {
+      if constexpr (SPLIT) {
+        // the ring as a split leaves its accumulator there: [piece of four columns][row], a warp's rows 512 bytes in a row
         if (ok) {
+          const uint32_t left = base + 16u * (uint32_t)row;
 #pragma unroll 1
           for (int c0 = 0; c0 < BF; c0 += 32) {
             uint32_t r[32];
@@ -784,33 +864,15 @@ q8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
         asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        if (kTileOutputs == 64 && ta.splits == 4)
+          finish_tokens<MODE, BF>(a, ta, ws, base, f0, tok0, rank, et);
+        else
+          drain<MODE, BF>(a, &map_y, ta.by_tma, ws, xs, f0, tok0, quad, lane, sender, out_smem, n_sent, rank, ta.splits, abort_flag,
+                          [&](int c0, uint32_t* r) { split_sum16(base + 16u * (uint32_t)row, ta.splits, c0, r); });
+      } else {
+        drain<MODE, BF>(a, &map_y, ta.by_tma, ws, xs, f0, tok0, quad, lane, sender, out_smem, n_sent, 0, 1, abort_flag,
+                        [&](int c0, uint32_t* r) { tmem_ld16(taddr + c0, r); });
       }
-      // 16 columns of this thread's token: the accumulator's, or the sum of all splits'
-      auto columns16 = [&](int c0, uint32_t* r) {
-        if (SPLIT) {
-          uint32_t v[kMaxSplits][16];  // the loads of all splits are in flight together
-#pragma unroll
-          for (int q = 0; q < kMaxSplits; ++q) {
-            if (q >= ta.splits) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[q][j] = 0;
-              continue;
-            }
-            uint32_t from;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(left + (uint32_t)(c0 / 4) * (BM * 16u)), "r"((uint32_t)q));
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[q][4 * c]), "=r"(v[q][4 * c + 1]),
-                           "=r"(v[q][4 * c + 2]), "=r"(v[q][4 * c + 3]) : "r"(from + (uint32_t)c * (BM * 16u)) : "memory");
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = v[0][j] + v[1][j] + v[2][j] + v[3][j];
-        } else {
-          tmem_ld16(taddr + c0, r);
-        }
-      };
-      drain<MODE, BF>(a, &map_y, ta.by_tma, ws, xs, f0, tok0, quad, lane, sender, out_smem, n_sent, rank, SPLIT ? ta.splits : 1, abort_flag,
-                      columns16);
       // this warp has read its lanes of the accumulator: hand it back to the MMA warp
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -1266,7 +1328,7 @@ double rows_ns(const RowsPlan& p, int M, int N, int K, bool gated, int bn, int s
 }
 // Tiles: a K block takes 370 / 245 / 205 at 256 / 128 / 64 columns, 540 / 300 / 205 where one tile of tokens reads each
 // weight once, from memory; a tile costs 5,200 / 3,450 / 2,800 beside its K blocks; a cluster's meetings and exchange
-// 2,900 (two blocks) or 4,200.  Tiles of two SMs (columns = 512): 335 a K block and 5,000 beside.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for
+// 2,900 (two blocks) or 4,200 (1,700 where a tile has 64 outputs).  Tiles of two SMs (columns = 512): 335 a K block and 5,000 beside.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for
 // 32 bytes of K: 39 against 30 us.)
 struct TilePlan { int columns, splits; double ns; };
 TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
@@ -1283,7 +1345,7 @@ TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
       const long long waves = (tiles * splits + sms - 1) / sms;
       double main = (double)((n_kb + splits - 1) / splits) * per_kb;
       if (waves > 1 && main < beside / 2) main = beside / 2;  // (the epilogue of all but the last tile runs beside the next)
-      const double ns = (double)waves * main + beside + (splits == 2 ? 2900 : splits == 4 ? 4200 : 0);
+      const double ns = (double)waves * main + beside + (splits == 2 ? 2900 : splits == 4 ? (outputs == 64 ? 1700 : 4200) : 0);
       if (best.ns == 0 || ns < best.ns) best = TilePlan{columns, splits, ns};
     }
   }
