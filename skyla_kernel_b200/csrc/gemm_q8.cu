@@ -1328,8 +1328,9 @@ double rows_ns(const RowsPlan& p, int M, int N, int K, bool gated, int bn, int s
 }
 // Tiles: a K block takes 370 / 245 / 205 at 256 / 128 / 64 columns, 540 / 300 / 205 where one tile of tokens reads each
 // weight once, from memory; a tile costs 5,200 / 3,450 / 2,800 beside its K blocks; a cluster's meetings and exchange
-// 2,900 (two blocks) or 4,200 (1,700 where a tile has 64 outputs).  Tiles of two SMs (columns = 512): 335 a K block and 5,000 beside.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for
-// 32 bytes of K: 39 against 30 us.)
+// 2,900 (two blocks) or 4,200 (1,700 where a tile has 64 outputs).  Tiles of two SMs (columns = 512): 335 a K block and
+// 5,000 beside.  (A gated product of 200 tokens by weight streaming, two instructions of 256 columns for 32 bytes of K:
+// 39 against 30 us.)
 struct TilePlan { int columns, splits; double ns; };
 TilePlan plan_tiles(int M, int N, int K, bool gated, int sms) {
   const long long n_kb = (K + KB - 1) / KB, n_t = (M + BM - 1) / BM;

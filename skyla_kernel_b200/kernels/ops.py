@@ -650,6 +650,19 @@ def _q8_dims(rows: Q8Rows, what: str, dims=_dims):
     return n, width, ld
 
 
+def _apart(a: torch.Tensor, lda: int, b: torch.Tensor, ldb: int) -> bool:
+    """Whether no element of ``a`` shares memory with one of ``b`` ([rows, width], the same rows; strides in elements).
+    Columns of one buffer count as apart where both step through it alike."""
+    n = a.shape[0]
+    sa, sb = a.element_size(), b.element_size()
+    pa, pb, wa, wb = a.data_ptr(), b.data_ptr(), a.shape[1] * sa, b.shape[1] * sb
+    if pa + (n - 1) * lda * sa + wa <= pb or pb + (n - 1) * ldb * sb + wb <= pa:
+        return True
+    step = lda * sa
+    off = (pb - pa) % step if step else 0
+    return n > 1 and step == ldb * sb and off >= wa and off + wb <= step
+
+
 def _device_of(first: torch.Tensor, *others) -> int:
     """The one CUDA device of the operands."""
     if not first.is_cuda:
@@ -761,6 +774,8 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         if m != n or w != width:
             raise KernelError(f"rmsnorm_q8: residual {tuple(residual.shape)} against x {tuple(x.shape)}")
         r_ptr, r_code = residual.data_ptr(), dtype_code(residual)
+        if not (r_ptr == x.data_ptr() and ldr == ld and r_code == code) and not _apart(x, ld, residual, ldr):
+            raise KernelError("rmsnorm_q8: the residual lies in x's memory, but is not x itself")
         dev = _device_of(x, weight, residual)
     if out is None:
         q, scale, ldq = _room(x, n, width)

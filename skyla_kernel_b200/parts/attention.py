@@ -29,7 +29,7 @@ from ..cache.kv import KVNeed
 from ..kernels import ops
 from ..weights.loader import TensorDecl
 from .base import NormedInput, Part, StepPlan, build_part, register_mixer
-from .linear import ACCUMULATE, STORE, Linear, layer_kernels, layer_linear
+from .linear import ACCUMULATE, STORE, Linear, layer_kernels, layer_linear, taken
 
 
 class DecodePages(StepPlan):
@@ -137,7 +137,7 @@ class GQAttention(Part):
         del parts
         self.qkv = layer_linear(fused, self.rt)
         self.q_only = self.qkv.first_outputs(self.nq * self.hd)
-        self.out = layer_linear(self.rt.matrix(tensors[t["o_proj"]]), self.rt)
+        self.out = layer_linear(self.rt.matrix(taken(tensors, t["o_proj"], self.rt)), self.rt)
         if self.qk_norm:
             self.q_norm_w = self.rt.vector(tensors[t["q_norm"]])
             self.k_norm_w = self.rt.vector(tensors[t["k_norm"]])

@@ -15,7 +15,7 @@ import torch
 from ..weights.loader import TensorDecl
 from ..kernels import ops
 from .base import NormedInput, Part, register_feed_forward
-from .linear import ACCUMULATE, GATED, Linear, layer_kernels, layer_linear
+from .linear import ACCUMULATE, GATED, Linear, layer_kernels, layer_linear, taken
 
 
 def fuse_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -50,7 +50,7 @@ class SwiGLU(Part):
         fused = fuse_gate_up(gate, up)
         del gate, up
         self.gate_up = layer_linear(self.rt.matrix(fused), self.rt, gated=True)
-        self.down = layer_linear(self.rt.matrix(tensors[t["down_proj"]]), self.rt)
+        self.down = layer_linear(self.rt.matrix(taken(tensors, t["down_proj"], self.rt)), self.rt)
 
     def kernels_needed(self):
         return tuple(dict.fromkeys(self.kernel_modules + layer_kernels(self.rt)))

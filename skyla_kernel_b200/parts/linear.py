@@ -204,6 +204,12 @@ def layer_linear(weight: torch.Tensor, rt, gated: bool = False):
     return Q8Linear(weight, rt, gated) if rt.int8 else Linear(weight, rt, gated)
 
 
+def taken(tensors, name: str, rt) -> torch.Tensor:
+    """A layer's matrix from the table that parts load from: taken out where its product keeps a copy in another form, so
+    that the original can be freed."""
+    return tensors.pop(name) if rt.int8 else tensors[name]
+
+
 def layer_kernels(rt):
     """The kernel libraries of :func:`layer_linear`'s products."""
     return Q8Linear.kernel_modules if rt.int8 else Linear.kernel_modules

@@ -56,6 +56,9 @@ def test_a_weight_is_kept_or_laid_out():
     lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), 1e-6, residual=torch.zeros(1, 8)),
     lambda: ops.rmsnorm_q8(torch.zeros(1, 8).expand(2, 8), torch.ones(8), 1e-6, residual=torch.zeros(2, 8)),
     lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), -1e-6),
+    lambda: (lambda t: ops.rmsnorm_q8(t[1:], torch.ones(8), 1e-6, residual=t[:3]))(torch.zeros(4, 8)),
+    lambda: (lambda t: ops.rmsnorm_q8(t[:, :8], torch.ones(8), 1e-6, residual=t[:, 4:12]))(torch.zeros(4, 16)),
+    lambda: (lambda t: ops.rmsnorm_q8(t, torch.ones(8), 1e-6, residual=t[:1].expand(4, 8)))(torch.zeros(4, 8)),
     lambda: ops.rmsnorm_q8(torch.zeros(2, 8), torch.ones(8), float("nan")),
     # product
     lambda: ops.linear_q8(_rows(2, 16), ops.Q8Weight(*_rows(4, 32)), torch.zeros(2, 4)),
@@ -77,6 +80,16 @@ def test_a_weight_is_kept_or_laid_out():
 def test_refusals(make):
     with pytest.raises(ops.KernelError):
         make()
+
+
+def test_what_shares_memory():
+    t = torch.zeros(6, 20)
+    apart = lambda a, b: ops._apart(a, a.stride(0), b, b.stride(0))  # noqa: E731
+    assert apart(t[:3], t[3:]) and apart(t[3:], t[:3]) and apart(t[:, :10], t[:, 10:]) and apart(t[:, 12:], t[:, :12])
+    assert not apart(t[:4], t[2:]) and not apart(t[:, :10], t[:, 9:19]) and not apart(t, t)
+    assert not apart(t[:3, :10], t[::2, 10:])                     # apart, but not by one step: counted as shared
+    assert not apart(t, t[:1].expand(6, 20)) and apart(t, torch.zeros(1, 20).expand(6, 20))
+    assert not apart(t[:1, :10], t[:1, 5:15]) and apart(t[:1, :10], t[:1, 10:])
 
 
 def test_too_many_elements_are_named():

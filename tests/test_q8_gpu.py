@@ -165,6 +165,11 @@ def test_a_residual_row_for_all_and_x_itself():
     _norm_close(x, weight, 1e-6, got)
     ops.rmsnorm_q8(x, weight, 1e-6, residual=x)
     assert torch.equal(x, 2 * want)
+    both = _rand(5, 224, seed=3)                      # x and residual as columns of one buffer
+    want = both[:, :96] + both[:, 128:]
+    got = ops.rmsnorm_q8(both[:, :96], weight, 1e-6, residual=both[:, 128:])
+    assert torch.equal(both[:, :96], want)
+    _norm_close(want, weight, 1e-6, got)
 
 
 def test_norm_rows_of_zeros_nans_and_overflow():
