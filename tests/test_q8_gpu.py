@@ -409,7 +409,7 @@ def test_a_run_of_the_operators(m):
 
 def test_two_streams_at_once():
     w = ops.Q8Weight.quantize(_rand(1024, 2048, seed=1))
-    xs = [ops.quantize_rows(_rand(m, 2048, seed=m)) for m in (8, 40, 129, 260)]
+    xs = [ops.quantize_rows(_rand(m, 2048, seed=m)) for m in (8, 40, 129, 260, 1500)]
     want = [_values(x, w) for x in xs]
     streams = [torch.cuda.Stream() for _ in xs]
     torch.cuda.synchronize()
