@@ -798,7 +798,7 @@ class Q8Weight:
     they wait for the kernels ahead of them, so it is finished for good: the constructor waits for the device (and
     refuses to run inside a stream capture), and nobody writes the tensors afterwards."""
 
-    __slots__ = ("rows", "gated", "n_out", "n_in", "ld")
+    __slots__ = ("rows", "gated", "n_out", "n_in", "ld", "_device", "_q", "_scale")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, gated: bool = False):
         n, width, ld = _q8_dims(Q8Rows(q, scale), "Q8Weight")
@@ -817,6 +817,9 @@ class Q8Weight:
             torch.cuda.synchronize(q.device)
         self.rows, self.gated, self.n_in, self.ld = Q8Rows(q, scale), bool(gated), width, ld
         self.n_out = n // 2 if gated else n
+        # what a launch needs of tensors that stay as they are: their device (None: the host) and where they lie
+        self._device = _device_of(q, scale) if q.is_cuda else None
+        self._q, self._scale = q.data_ptr(), scale.data_ptr()
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, gated: bool = False) -> "Q8Weight":
@@ -842,7 +845,6 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
     of a gated weight, bfloat16).  ``x``'s rows should begin on multiples of 16 bytes (as :func:`q8_rows` makes
     them): others run on the plain kernel, with the same results."""
     q, scale = x
-    rows = w.rows
     m, k, ldx = _q8_dims(x, "linear_q8")
     if k != w.n_in:
         raise KernelError(f"linear_q8: tokens of {k} against a weight of {w.n_in} inputs")
@@ -854,7 +856,9 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
     if code != (F32 if mode == ACCUMULATE else BF16 if mode == GATED else code):
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
-    dev = _device_of(q, scale, rows.q, rows.scale, y)
+    dev = _device_of(q, scale, y)
+    if dev != w._device:
+        raise KernelError(f"linear_q8: tokens on {q.device}, the weight on {w.rows.q.device}")
     if state is None:
         flag = _default_flag(dev)
     else:
@@ -864,11 +868,9 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         ldx = w.ld  # the distance to a next row that is not there
     if ldx % 16 == 0 and ldx >= k and q.data_ptr() % 16 == 0:
         epilogue = TC_ACCUM_F32 if mode == ACCUMULATE else TC_GLU_BF16 if mode == GATED else TC_STORE_F32 if code == F32 else TC_STORE_BF16
-        _linear_q8(dev, q.data_ptr(), ldx, scale.data_ptr(), rows.q.data_ptr(), w.ld, rows.scale.data_ptr(), m, yn, k, y.data_ptr(), ldy,
-                   epilogue, flag.data_ptr())
+        _linear_q8(dev, q.data_ptr(), ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y.data_ptr(), ldy, epilogue, flag.data_ptr())
     else:
-        _linear_q8_plain(dev, q.data_ptr(), ldx, scale.data_ptr(), rows.q.data_ptr(), w.ld, rows.scale.data_ptr(), m, yn, k, y.data_ptr(),
-                         code, ldy, mode)
+        _linear_q8_plain(dev, q.data_ptr(), ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y.data_ptr(), code, ldy, mode)
     return y
 
 
