@@ -663,6 +663,12 @@ def _apart(a: torch.Tensor, lda: int, b: torch.Tensor, ldb: int) -> bool:
     return n > 1 and step == ldb * sb and off >= wa and off + wb <= step
 
 
+def _keep_apart(out: torch.Tensor, ldo: int, x: torch.Tensor, ldx: int, what: str) -> None:
+    """Refuses an output in the memory of an input: other blocks still read what one would write."""
+    if x.numel() and not _apart(out, ldo, x, ldx):
+        raise KernelError(f"{what}: the output lies in the input's memory")
+
+
 def _device_of(first: torch.Tensor, *others) -> int:
     """The one CUDA device of the operands."""
     if not first.is_cuda:
@@ -722,7 +728,7 @@ _linear_q8_plain = _Launcher("linear_q8_plain", "skyla_linear_q8_plain", c_void_
 
 def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
     """Each row of ``x`` (bfloat16 or float32, [rows, width]) in 8 bits: ``scale = max|x| / 127`` and
-    ``q = x / scale``, the exact quotient rounded to the nearest integer (ties to even).
+    ``q = x / scale``, the exact quotient rounded to the nearest integer (ties to even).  ``out`` lies apart from ``x``.
 
     A row of zeros stays zeros; a row that holds a NaN or an infinity gets the scale NaN and zeros."""
     n, width, ld = _dims(x, "quantize_rows")
@@ -736,19 +742,23 @@ def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
         m, w, ldq = _q8_dims(out, "quantize_rows", _written_dims)
         if m != n or w != width:
             raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
+        _keep_apart(q, ldq, x, ld, "quantize_rows")
         dev = _device_of(x, q, scale)
     _quantize_rows(dev, x.data_ptr(), code, ld, n, width, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
 
 def dequantize_rows(rows: Q8Rows, out: torch.Tensor) -> torch.Tensor:
-    """What 8-bit rows stand for: ``out[r] = q[r] * scale[r]`` in ``out``'s type (bfloat16 or float32)."""
+    """What 8-bit rows stand for: ``out[r] = q[r] * scale[r]`` in ``out``'s type (bfloat16 or float32), apart from ``rows``."""
     q, scale = rows
     n, width, ldq = _q8_dims(rows, "dequantize_rows")
     m, w, ldo = _written_dims(out, "dequantize_rows")
     if m != n or w != width:
         raise KernelError(f"dequantize_rows: rows {tuple(q.shape)} do not go into {tuple(out.shape)}")
-    _dequantize_rows(_device_of(q, scale, out), q.data_ptr(), ldq, scale.data_ptr(), n, width, out.data_ptr(), dtype_code(out), ldo)
+    q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
+    if o_ptr < q_ptr + n * ldq + width and q_ptr < o_ptr + 4 * n * ldo:
+        _keep_apart(out, ldo, q, ldq, "dequantize_rows")
+    _dequantize_rows(_device_of(q, scale, out), q_ptr, ldq, scale.data_ptr(), n, width, o_ptr, dtype_code(out), ldo)
     return out
 
 
@@ -756,7 +766,7 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
                residual: Optional[torch.Tensor] = None) -> Q8Rows:
     """``rmsnorm(x) * weight`` in 8-bit rows, computed in 32 bits; with ``residual`` the rows are added into ``x``
     first (``x`` is written, in its own type, and the norm is that of the sum as it is kept).  ``residual`` is ``x``
-    itself or lies apart from it.
+    itself or lies apart from it; ``out`` lies apart from both.
 
     ``x`` and ``residual``: bfloat16 or float32.  A row whose sum of squares or whose products with the weight
     leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row of zeros with ``eps = 0``."""
@@ -768,7 +778,6 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         raise KernelError(f"rmsnorm_q8: eps must not be negative, got {eps}")
     if residual is None:
         r_ptr, r_code, ldr = None, 0, 0
-        dev = _device_of(x, weight)
     else:
         m, w, ldr = _dims(residual, "rmsnorm_q8")
         if m != n or w != width:
@@ -776,8 +785,8 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         r_ptr, r_code = residual.data_ptr(), dtype_code(residual)
         if not (r_ptr == x.data_ptr() and ldr == ld and r_code == code) and not _apart(x, ld, residual, ldr):
             raise KernelError("rmsnorm_q8: the residual lies in x's memory, but is not x itself")
-        dev = _device_of(x, weight, residual)
     if out is None:
+        dev = _device_of(x, weight) if residual is None else _device_of(x, weight, residual)
         q, scale, ldq = _room(x, n, width)
         out = Q8Rows(q, scale)
     else:
@@ -785,7 +794,10 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         m, w, ldq = _q8_dims(out, "rmsnorm_q8", _written_dims)
         if m != n or w != width:
             raise KernelError(f"rmsnorm_q8: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
-        _device_of(x, q, scale)
+        _keep_apart(q, ldq, x, ld, "rmsnorm_q8")
+        if residual is not None:
+            _keep_apart(q, ldq, residual, ldr, "rmsnorm_q8")
+        dev = _device_of(x, weight, q, scale, x if residual is None else residual)
     _rmsnorm_q8(dev, x.data_ptr(), code, ld, r_ptr, r_code, ldr, n, width, weight.data_ptr(), eps, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
@@ -842,8 +854,8 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
     the sum exact, the scales applied in 32 bits.
 
     ``mode``: STORE (``y = v``, bfloat16 or float32), ACCUMULATE (``y += v``, float32), GATED (``y = silu(gate) * up``
-    of a gated weight, bfloat16).  ``x``'s rows should begin on multiples of 16 bytes (as :func:`q8_rows` makes
-    them): others run on the plain kernel, with the same results."""
+    of a gated weight, bfloat16).  ``y`` lies apart from ``x``.  ``x``'s rows should begin on multiples of 16 bytes
+    (as :func:`q8_rows` makes them): others run on the plain kernel, with the same results."""
     q, scale = x
     m, k, ldx = _q8_dims(x, "linear_q8")
     if k != w.n_in:
@@ -856,6 +868,9 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
     if code != (F32 if mode == ACCUMULATE else BF16 if mode == GATED else code):
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
+    q_ptr, y_ptr = q.data_ptr(), y.data_ptr()
+    if y_ptr < q_ptr + m * ldx + k and q_ptr < y_ptr + 4 * m * ldy:  # (a first look, cheaper than the whole one)
+        _keep_apart(y, ldy, q, ldx, "linear_q8")
     dev = _device_of(q, scale, y)
     if dev != w._device:
         raise KernelError(f"linear_q8: tokens on {q.device}, the weight on {w.rows.q.device}")
@@ -866,11 +881,11 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         _device_of(y, flag)
     if m == 1:
         ldx = w.ld  # the distance to a next row that is not there
-    if ldx % 16 == 0 and ldx >= k and q.data_ptr() % 16 == 0:
+    if ldx % 16 == 0 and ldx >= k and q_ptr % 16 == 0:
         epilogue = TC_ACCUM_F32 if mode == ACCUMULATE else TC_GLU_BF16 if mode == GATED else TC_STORE_F32 if code == F32 else TC_STORE_BF16
-        _linear_q8(dev, q.data_ptr(), ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y.data_ptr(), ldy, epilogue, flag.data_ptr())
+        _linear_q8(dev, q_ptr, ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y_ptr, ldy, epilogue, flag.data_ptr())
     else:
-        _linear_q8_plain(dev, q.data_ptr(), ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y.data_ptr(), code, ldy, mode)
+        _linear_q8_plain(dev, q_ptr, ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y_ptr, code, ldy, mode)
     return y
 
 

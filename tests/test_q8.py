@@ -92,6 +92,23 @@ def test_what_shares_memory():
     assert not apart(t[:1, :10], t[:1, 5:15]) and apart(t[:1, :10], t[:1, 10:])
 
 
+def test_outputs_in_the_memory_of_inputs_are_refused():
+    t = torch.zeros(4, 32)
+    inside = lambda n, k: ops.Q8Rows(t.view(torch.int8)[:n, 4:4 + k], torch.ones(n))  # noqa: E731
+    for call in (lambda: ops.quantize_rows(t[:, :8], inside(4, 8)),
+                 lambda: ops.quantize_rows(t[:1], inside(1, 32)),
+                 lambda: ops.quantize_rows(t[:1].expand(4, 32), inside(4, 32)),
+                 lambda: ops.rmsnorm_q8(t, torch.ones(32), 1e-6, inside(4, 32)),
+                 lambda: ops.rmsnorm_q8(torch.zeros(4, 32), torch.ones(32), 1e-6, inside(4, 32), residual=t),
+                 lambda: ops.dequantize_rows(inside(4, 32), t),
+                 lambda: ops.linear_q8(inside(4, 16), ops.Q8Weight(*_rows(32, 16)), t)):
+        with pytest.raises(ops.KernelError, match="input's memory"):
+            call()
+    # beside one another in one buffer they are apart: what is refused then is only that there is no GPU
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.quantize_rows(t[:, 9:], inside(4, 23))
+
+
 def test_too_many_elements_are_named():
     for shape in ((1, 2 ** 31), (2 ** 31, 2)):
         with pytest.raises(ops.KernelError, match="2\\^29"):
