@@ -833,6 +833,11 @@ class Q8Weight:
         self._device = _device_of(q, scale) if q.is_cuda else None
         self._q, self._scale = q.data_ptr(), scale.data_ptr()
 
+    def __reduce__(self):
+        """A copy, a pickled or a saved weight is laid out and waited for like any other: what ``__slots__`` hold
+        beside the tensors is true of these tensors alone."""
+        return type(self), (*self.rows, self.gated)
+
     @classmethod
     def quantize(cls, weight: torch.Tensor, gated: bool = False) -> "Q8Weight":
         """A bfloat16 or float32 weight in 8 bits, each row (output) with its own scale."""
