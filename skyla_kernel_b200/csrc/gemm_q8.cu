@@ -24,6 +24,7 @@ SKYLA_EXPORT_ERROR_MESSAGE()
 namespace {
 using namespace skyla::tc;
 using skyla::q8::scaled;
+using skyla::q8::silu_times;
 
 enum Mode : int { kStoreBf16 = 0, kStoreF32 = 1, kAccumF32 = 2, kGluBf16 = 3 };
 
@@ -67,9 +68,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&p);
 }
-// With the fast exponential and division: their error (a few 2^-22, 2^-17 far from zero) is well below the
-// bfloat16 rounding that follows.
-__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // ---------------------------------------------------------------------------------- few tokens: weight streaming
 // The structure of the bfloat16 kernel of the same kind (gemm_tc.cu, where its measurements stand): one box brings

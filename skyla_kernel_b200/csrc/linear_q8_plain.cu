@@ -7,6 +7,7 @@
 #include "q8.cuh"
 using namespace skyla;
 using skyla::q8::scaled;
+using skyla::q8::silu_times;
 SKYLA_EXPORT_ERROR_MESSAGE()
 
 namespace {
@@ -83,8 +84,7 @@ __global__ void __launch_bounds__(kThreads) linear_q8_plain_kernel(Args a) {
       TY* y = (TY*)a.y + t * a.ldy + f;
       const float v = scaled(acc[i][j], sx, a.w_scale[f]);
       if (MODE == kGated) {
-        const float u = scaled(up[i][j], sx, a.w_scale[a.n + f]);
-        *y = from_float<TY>(v / (1.0f + expf(-v)) * u);
+        *y = from_float<TY>(silu_times(v, scaled(up[i][j], sx, a.w_scale[a.n + f])));
       } else if (MODE == kAccumulate) {
         *y = from_float<TY>(__fadd_rn(to_float(*y), v));
       } else {
