@@ -14,6 +14,7 @@
 // land, frees its TMEM and returns.
 #include <cuda.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "q8.cuh"
@@ -1133,24 +1134,38 @@ int current_device() {
   cudaGetDevice(&dev);
   return dev >= 0 && dev < kMaxDevices ? dev : 0;
 }
-int sm_count() {
-  static int n[kMaxDevices] = {};
-  const int dev = current_device();
-  if (n[dev] == 0) {
-    int v = 0;
-    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-    n[dev] = v > 0 ? v : 148;
+// What a device answers to a question, asked once.  Threads that come first together ask each for themselves; the answer
+// that is stored first is everybody's, so that a plan and its launch go by the same one.
+struct Asked {
+  std::atomic<int> known[kMaxDevices];  // the answer + 1
+  template <typename Ask>
+  int operator()(Ask ask) {
+    std::atomic<int>& k = known[current_device()];
+    int v = k.load();
+    if (v == 0) {
+      const int mine = 1 + ask();
+      if (k.compare_exchange_strong(v, mine)) v = mine;
+    }
+    return v - 1;
   }
-  return n[dev];
+};
+int sm_count() {
+  static Asked asked;
+  return asked([] {
+    int v = 0;
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, current_device());
+    return v > 0 ? v : 148;
+  });
 }
 // Shared memory of a kernel, reserved once per device.
+typedef std::atomic<bool> Done[kMaxDevices];
 template <typename K>
-int reserve(K kernel, int bytes, bool* done) {
+int reserve(K kernel, int bytes, Done& done) {
   const int dev = current_device();
-  if (done[dev]) return kOk;
+  if (done[dev].load()) return kOk;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(kLaunchFailed, "linear_q8: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-  done[dev] = true;
+  done[dev].store(true);
   return kOk;
 }
 
@@ -1158,13 +1173,10 @@ struct RowsPlan { int rows, splits, kkb, kstack; };
 
 // How many clusters of `size` blocks run at a time (one block per SM, clusters inside a GPC).
 int cluster_room(int size) {
-  static int room[kMaxDevices][2] = {};
-  const int dev = current_device();
-  int& n = room[dev][size == 4];
-  if (n == 0) {
+  static Asked asked[2];
+  return asked[size == 4]([size] {
     auto kernel = q8_rows_kernel<64, kAccumF32, kCluster>;
-    static bool done[kMaxDevices] = {};
-    n = -1;
+    static Done done;
     if (reserve(kernel, kRowsSmemBytes, done) != kOk) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1024, 1, size);
@@ -1178,10 +1190,10 @@ int cluster_room(int size) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int v = 0;
-    if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) == cudaSuccess && v > 0) n = v;
-    else cudaGetLastError();
-  }
-  return n > 0 ? n : 0;
+    if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) == cudaSuccess) return v > 0 ? v : 0;
+    cudaGetLastError();
+    return 0;
+  });
 }
 
 // The tile height is the smallest multiple of 8 whose tiles fill the SMs in whole waves.  Up to 16 tokens, tiles of at
@@ -1271,17 +1283,17 @@ int launch_rows(const Operands& o, const Args& a, const RowsPlan& p, cudaStream_
   const int smem = fixed + ra.n_stages * stage;
   const dim3 grid((unsigned)((a.N + p.rows - 1) / p.rows), 1, (unsigned)p.splits);
   if (p.splits > 1) {
-    static bool done[kMaxDevices] = {};
+    static Done done;
     auto kernel = q8_rows_kernel<BN, M2, kCluster>;
     if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
     launch_overlapped_cluster(kernel, grid, dim3(kThreads), (size_t)smem, stream, (unsigned)p.splits, mw, mx, a, ra);
   } else if (p.kstack > 1) {
-    static bool done[kMaxDevices] = {};
+    static Done done;
     auto kernel = q8_rows_kernel<16, M2, kStacked>;
     if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
     launch_overlapped(kernel, grid, dim3(kThreads), (size_t)smem, stream, mw, mx, a, ra);
   } else {
-    static bool done[kMaxDevices] = {};
+    static Done done;
     auto kernel = q8_rows_kernel<BN, MODE, kPlain>;
     if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
     launch_overlapped(kernel, grid, dim3(kThreads), (size_t)smem, stream, mw, mx, a, ra);
@@ -1291,12 +1303,10 @@ int launch_rows(const Operands& o, const Args& a, const RowsPlan& p, cudaStream_
 
 // How many pairs of blocks run at a time.
 int pair_room() {
-  static int room[kMaxDevices] = {};
-  int& n = room[current_device()];
-  if (n == 0) {
+  static Asked asked;
+  return asked([] {
     auto kernel = q8_pair_kernel<kStoreBf16>;
-    static bool done[kMaxDevices] = {};
-    n = -1;
+    static Done done;
     if (reserve(kernel, kPairSmemBytes, done) != kOk) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2048);
@@ -1309,10 +1319,10 @@ int pair_room() {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int v = 0;
-    if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) == cudaSuccess && v > 0) n = v;
-    else cudaGetLastError();
-  }
-  return n > 0 ? n : 0;
+    if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) == cudaSuccess) return v > 0 ? v : 0;
+    cudaGetLastError();
+    return 0;
+  });
 }
 
 // What the three kernels were measured to take, in nanoseconds, for products of 17 to 2,048 tokens and the layer sizes
@@ -1419,7 +1429,7 @@ int launch_tiles(const Operands& o, const Args& a, int splits, cudaStream_t stre
   if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, ta.x_rows, kkb)) return rc;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, MODE == kGluBf16 ? BF / 2 : BF, kkb)) return rc;
   if (int rc = output_map(&my, mx, a, f32, &ta.by_tma)) return rc;
-  static bool done[kMaxDevices] = {};
+  static Done done;
   auto kernel = q8_tile_kernel<MODE, BF, SPLIT>;
   if (int rc = reserve(kernel, C::kSmemBytes, done)) return rc;
   const int sms = sm_count();
@@ -1446,7 +1456,7 @@ int launch_pairs(const Operands& o, const Args& a, cudaStream_t stream) {
   if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BM, 1)) return rc;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, BM, 1)) return rc;
   if (int rc = output_map(&my, mx, a, MODE == kStoreF32 || MODE == kAccumF32, &ta.by_tma)) return rc;
-  static bool done[kMaxDevices] = {};
+  static Done done;
   auto kernel = q8_pair_kernel<MODE>;
   if (int rc = reserve(kernel, kPairSmemBytes, done)) return rc;
   const long long room = pair_room();
