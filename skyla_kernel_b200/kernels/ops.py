@@ -245,7 +245,7 @@ def default_state(device) -> KernelState:
         dev = torch.device(dev.type, torch.cuda.current_device())
     st = _DEFAULT_STATES.get(dev)
     if st is None:
-        st = _DEFAULT_STATES[dev] = KernelState(dev)
+        st = _DEFAULT_STATES.setdefault(dev, KernelState(dev))  # (one for all threads that come first together)
     return st
 
 

@@ -122,3 +122,31 @@ def test_what_a_runtime_takes():
         Runtime(torch.device("cpu"), "float32", weights="int8")
     with pytest.raises(ValueError):
         Runtime(torch.device("cpu"), "bfloat16", weights="int4")
+
+
+def test_one_error_word_for_threads_that_come_first_together(monkeypatch):
+    """The word that the product's kernels write is the one that ``check_device_errors`` reads."""
+    import threading
+    import time
+
+    class Slow:
+        def __init__(self, device):
+            time.sleep(0.02)
+            self.error_flag = torch.zeros(1, dtype=torch.int32)
+
+    monkeypatch.setattr(ops, "KernelState", Slow)
+    monkeypatch.setattr(ops, "_DEFAULT_STATES", {})
+    monkeypatch.setattr(ops, "_FLAGS", {})
+    start, got = threading.Barrier(8), []
+
+    def ask():
+        start.wait()
+        got.append(ops._default_flag(0))
+
+    threads = [threading.Thread(target=ask) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    read = ops.default_state("cuda:0").error_flag
+    assert len(got) == 8 and all(flag is read for flag in [*got, ops._default_flag(0)])
