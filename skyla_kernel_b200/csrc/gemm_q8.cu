@@ -1252,7 +1252,6 @@ template <int BN, int MODE>
 int launch_rows(const Operands& o, const Args& a, const RowsPlan& p, cudaStream_t stream) {
   constexpr bool gated = MODE == kGluBf16;
   constexpr int kATiles = gated ? 2 : 1;
-  constexpr int M2 = gated ? kStoreBf16 : MODE;  // (no gated instance of the cluster and stacked kernels is built)
   CUtensorMap mw, mx;
   if (int rc = rows_map(&mw, o.w, o.ldw, o.w_rows, a.K, p.rows, p.kkb)) return rc;
   if (int rc = rows_map(&mx, o.x, o.ldx, a.M, a.K, BN, p.kkb)) return rc;
@@ -1282,16 +1281,25 @@ int launch_rows(const Operands& o, const Args& a, const RowsPlan& p, cudaStream_
     return fail(kBadArgument, "linear_q8: %d splits leave one without K blocks", p.splits);
   const int smem = fixed + ra.n_stages * stage;
   const dim3 grid((unsigned)((a.N + p.rows - 1) / p.rows), 1, (unsigned)p.splits);
+  // (plan_rows stacks K blocks up to 16 tokens only and cuts K beyond only, neither for a gated weight)
   if (p.splits > 1) {
-    static Done done;
-    auto kernel = q8_rows_kernel<BN, M2, kCluster>;
-    if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
-    launch_overlapped_cluster(kernel, grid, dim3(kThreads), (size_t)smem, stream, (unsigned)p.splits, mw, mx, a, ra);
+    if constexpr (!gated && BN > 16) {
+      static Done done;
+      auto kernel = q8_rows_kernel<BN, MODE, kCluster>;
+      if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
+      launch_overlapped_cluster(kernel, grid, dim3(kThreads), (size_t)smem, stream, (unsigned)p.splits, mw, mx, a, ra);
+    } else {
+      return fail(kBadArgument, "linear_q8: %d splits of K for tiles of %d tokens", p.splits, BN);
+    }
   } else if (p.kstack > 1) {
-    static Done done;
-    auto kernel = q8_rows_kernel<16, M2, kStacked>;
-    if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
-    launch_overlapped(kernel, grid, dim3(kThreads), (size_t)smem, stream, mw, mx, a, ra);
+    if constexpr (!gated && BN == 16) {
+      static Done done;
+      auto kernel = q8_rows_kernel<BN, MODE, kStacked>;
+      if (int rc = reserve(kernel, kRowsSmemBytes, done)) return rc;
+      launch_overlapped(kernel, grid, dim3(kThreads), (size_t)smem, stream, mw, mx, a, ra);
+    } else {
+      return fail(kBadArgument, "linear_q8: %d K blocks stacked for tiles of %d tokens", p.kstack, BN);
+    }
   } else {
     static Done done;
     auto kernel = q8_rows_kernel<BN, MODE, kPlain>;
