@@ -669,6 +669,20 @@ def _keep_apart(out: torch.Tensor, ldo: int, x: torch.Tensor, ldx: int, what: st
         raise KernelError(f"{what}: the output lies in the input's memory")
 
 
+def _keep_vector_apart(t: torch.Tensor, ld: int, v: torch.Tensor, what: str) -> None:
+    """Refuses a contiguous vector (scales, a norm's weight) in the memory of a matrix, one of which is written.
+    Between the rows, or behind the columns that ``t`` has of its buffer, it is apart."""
+    size = t.element_size()
+    p, v_ptr = t.data_ptr(), v.data_ptr()
+    n, width = t.shape
+    step, width, length = ld * size, width * size, v.numel() * v.element_size()
+    if v_ptr >= p + (n - 1) * step + width or p >= v_ptr + length or not t.numel():
+        return
+    off = (v_ptr - p) % step if step else 0
+    if v_ptr < p or off < width or off + length > step:
+        raise KernelError(f"{what}: an output lies in another operand's memory")
+
+
 def _device_of(first: torch.Tensor, *others) -> int:
     """The one CUDA device of the operands."""
     if not first.is_cuda:
@@ -743,6 +757,12 @@ def quantize_rows(x: torch.Tensor, out: Optional[Q8Rows] = None) -> Q8Rows:
         if m != n or w != width:
             raise KernelError(f"quantize_rows: rows {tuple(x.shape)} do not go into {tuple(q.shape)}")
         _keep_apart(q, ldq, x, ld, "quantize_rows")
+        x_ptr, q_ptr, s_ptr = x.data_ptr(), q.data_ptr(), scale.data_ptr()
+        s_end = s_ptr + 4 * n
+        x_end = x_ptr + 4 * n * ld + 4 * width
+        if (x_ptr < s_end and s_ptr < x_end) or (q_ptr < s_end and s_ptr < q_ptr + n * ldq):  # (a first look)
+            _keep_vector_apart(x, ld, scale, "quantize_rows")
+            _keep_vector_apart(q, ldq, scale, "quantize_rows")
         dev = _device_of(x, q, scale)
     _quantize_rows(dev, x.data_ptr(), code, ld, n, width, q.data_ptr(), ldq, scale.data_ptr())
     return out
@@ -758,6 +778,7 @@ def dequantize_rows(rows: Q8Rows, out: torch.Tensor) -> torch.Tensor:
     q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
     if o_ptr < q_ptr + n * ldq + width and q_ptr < o_ptr + 4 * n * ldo:
         _keep_apart(out, ldo, q, ldq, "dequantize_rows")
+    _keep_vector_apart(out, ldo, scale, "dequantize_rows")
     _dequantize_rows(_device_of(q, scale, out), q_ptr, ldq, scale.data_ptr(), n, width, o_ptr, dtype_code(out), ldo)
     return out
 
@@ -766,7 +787,7 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
                residual: Optional[torch.Tensor] = None) -> Q8Rows:
     """``rmsnorm(x) * weight`` in 8-bit rows, computed in 32 bits; with ``residual`` the rows are added into ``x``
     first (``x`` is written, in its own type, and the norm is that of the sum as it is kept).  ``residual`` is ``x``
-    itself or lies apart from it; ``out`` lies apart from both.
+    itself or lies apart from it; what is written lies apart from ``weight``, ``out`` from all others.
 
     ``x`` and ``residual``: bfloat16 or float32.  A row whose sum of squares or whose products with the weight
     leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row of zeros with ``eps = 0``."""
@@ -776,6 +797,8 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         raise KernelError(f"rmsnorm_q8: the weight must be a contiguous float32 vector of {width}")
     if not eps >= 0:
         raise KernelError(f"rmsnorm_q8: eps must not be negative, got {eps}")
+    x_ptr, w_ptr = x.data_ptr(), weight.data_ptr()
+    x_end, w_end = x_ptr + 4 * n * ld + 4 * width, w_ptr + 4 * width
     if residual is None:
         r_ptr, r_code, ldr = None, 0, 0
     else:
@@ -783,8 +806,10 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         if m != n or w != width:
             raise KernelError(f"rmsnorm_q8: residual {tuple(residual.shape)} against x {tuple(x.shape)}")
         r_ptr, r_code = residual.data_ptr(), dtype_code(residual)
-        if not (r_ptr == x.data_ptr() and ldr == ld and r_code == code) and not _apart(x, ld, residual, ldr):
+        if not (r_ptr == x_ptr and ldr == ld and r_code == code) and not _apart(x, ld, residual, ldr):
             raise KernelError("rmsnorm_q8: the residual lies in x's memory, but is not x itself")
+        if x_ptr < w_end and w_ptr < x_end:  # (a first look, cheaper than the whole one)
+            _keep_vector_apart(x, ld, weight, "rmsnorm_q8")
     if out is None:
         dev = _device_of(x, weight) if residual is None else _device_of(x, weight, residual)
         q, scale, ldq = _room(x, n, width)
@@ -797,8 +822,17 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
         _keep_apart(q, ldq, x, ld, "rmsnorm_q8")
         if residual is not None:
             _keep_apart(q, ldq, residual, ldr, "rmsnorm_q8")
+            _keep_vector_apart(residual, ldr, scale, "rmsnorm_q8")
+        q_ptr, s_ptr = q.data_ptr(), scale.data_ptr()
+        q_end, s_end = q_ptr + n * ldq, s_ptr + 4 * n
+        if ((x_ptr < s_end and s_ptr < x_end) or (q_ptr < s_end and s_ptr < q_end) or (q_ptr < w_end and w_ptr < q_end)
+                or (w_ptr < s_end and s_ptr < w_end)):  # (a first look)
+            _keep_vector_apart(x, ld, scale, "rmsnorm_q8")
+            _keep_vector_apart(q, ldq, scale, "rmsnorm_q8")
+            _keep_vector_apart(q, ldq, weight, "rmsnorm_q8")
+            _keep_vector_apart(weight[None], width, scale, "rmsnorm_q8")
         dev = _device_of(x, weight, q, scale, x if residual is None else residual)
-    _rmsnorm_q8(dev, x.data_ptr(), code, ld, r_ptr, r_code, ldr, n, width, weight.data_ptr(), eps, q.data_ptr(), ldq, scale.data_ptr())
+    _rmsnorm_q8(dev, x_ptr, code, ld, r_ptr, r_code, ldr, n, width, w_ptr, eps, q.data_ptr(), ldq, scale.data_ptr())
     return out
 
 
@@ -873,9 +907,12 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         raise KernelError(f"linear_q8: y {tuple(y.shape)} is not [{m}, {w.n_out}]")
     if code != (F32 if mode == ACCUMULATE else BF16 if mode == GATED else code):
         raise KernelError(f"linear_q8: mode {mode} does not write {y.dtype}")
-    q_ptr, y_ptr = q.data_ptr(), y.data_ptr()
-    if y_ptr < q_ptr + m * ldx + k and q_ptr < y_ptr + 4 * m * ldy:  # (a first look, cheaper than the whole one)
+    q_ptr, y_ptr, s_ptr = q.data_ptr(), y.data_ptr(), scale.data_ptr()
+    y_end = y_ptr + 4 * m * ldy
+    if y_ptr < q_ptr + m * ldx + k and q_ptr < y_end:  # (a first look, cheaper than the whole one)
         _keep_apart(y, ldy, q, ldx, "linear_q8")
+    if y_ptr < s_ptr + 4 * m and s_ptr < y_end:
+        _keep_vector_apart(y, ldy, scale, "linear_q8")
     dev = _device_of(q, scale, y)
     if dev != w._device:
         raise KernelError(f"linear_q8: tokens on {q.device}, the weight on {w.rows.q.device}")
@@ -888,9 +925,9 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
         ldx = w.ld  # the distance to a next row that is not there
     if ldx % 16 == 0 and ldx >= k and q_ptr % 16 == 0:
         epilogue = TC_ACCUM_F32 if mode == ACCUMULATE else TC_GLU_BF16 if mode == GATED else TC_STORE_F32 if code == F32 else TC_STORE_BF16
-        _linear_q8(dev, q_ptr, ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y_ptr, ldy, epilogue, flag.data_ptr())
+        _linear_q8(dev, q_ptr, ldx, s_ptr, w._q, w.ld, w._scale, m, yn, k, y_ptr, ldy, epilogue, flag.data_ptr())
     else:
-        _linear_q8_plain(dev, q_ptr, ldx, scale.data_ptr(), w._q, w.ld, w._scale, m, yn, k, y_ptr, code, ldy, mode)
+        _linear_q8_plain(dev, q_ptr, ldx, s_ptr, w._q, w.ld, w._scale, m, yn, k, y_ptr, code, ldy, mode)
     return y
 
 

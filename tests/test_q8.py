@@ -150,3 +150,38 @@ def test_one_error_word_for_threads_that_come_first_together(monkeypatch):
         t.join()
     read = ops.default_state("cuda:0").error_flag
     assert len(got) == 8 and all(flag is read for flag in [*got, ops._default_flag(0)])
+
+
+def _packed(n, k, at, buf):
+    """8-bit rows whose scales begin at byte ``at`` of ``buf``; the integers lie elsewhere."""
+    return ops.Q8Rows(torch.zeros(n, k, dtype=torch.int8), buf.view(-1).view(torch.int8)[at:at + 4 * n].view(torch.float32))
+
+
+def test_scales_in_the_memory_of_other_operands_are_refused():
+    t = torch.zeros(4, 32)
+    q = lambda n, k: t.view(torch.int8)[:n, :k]  # noqa: E731
+    flat = t.view(-1)
+    for call in (lambda: ops.quantize_rows(t, _packed(4, 32, 16, t)),
+                 lambda: ops.quantize_rows(t[:, :8], _packed(4, 8, 24, t)),                    # across the end of a row
+                 lambda: ops.quantize_rows(torch.zeros(4, 8), ops.Q8Rows(q(4, 8), flat[:4])),  # the rows' own scales
+                 lambda: ops.dequantize_rows(_packed(4, 32, 0, t), t),
+                 lambda: ops.rmsnorm_q8(t, torch.ones(32), 1e-6, _packed(4, 32, 16, t)),
+                 lambda: ops.rmsnorm_q8(torch.zeros(4, 32), torch.ones(32), 1e-6, _packed(4, 32, 16, t), residual=t),
+                 lambda: ops.rmsnorm_q8(torch.zeros(4, 32), flat[:32], 1e-6, _packed(4, 32, 16, t)),
+                 lambda: ops.rmsnorm_q8(torch.zeros(4, 32), flat[:32], 1e-6, ops.Q8Rows(q(4, 32), torch.ones(4))),
+                 lambda: ops.rmsnorm_q8(torch.zeros(4, 32), torch.ones(32), 1e-6, ops.Q8Rows(q(4, 32), flat[:4])),
+                 lambda: ops.rmsnorm_q8(t, flat[32:64], 1e-6, residual=torch.zeros(4, 32)),    # the weight in rows that are written
+                 lambda: ops.linear_q8(_packed(4, 16, 128, t), ops.Q8Weight(*_rows(32, 16)), t)):
+        with pytest.raises(ops.KernelError, match="memory"):
+            call()
+    # behind the columns that are used they are apart: what is refused then is only that there is no GPU
+    for call in (lambda: ops.quantize_rows(t[:, :8], _packed(4, 8, 32, t)),
+                 lambda: ops.quantize_rows(t[1:], _packed(3, 32, 0, t)),
+                 lambda: ops.quantize_rows(t[:3], _packed(3, 32, 4 * 96, t)),
+                 lambda: ops.dequantize_rows(_packed(4, 8, 32, t), t[:, :8]),
+                 lambda: ops.rmsnorm_q8(t[:, :8], flat[8:16], 1e-6, residual=torch.zeros(4, 8)),
+                 lambda: ops.rmsnorm_q8(t, flat[32:64], 1e-6),
+                 lambda: ops.linear_q8(_packed(4, 16, 32, t), ops.Q8Weight(*_rows(8, 16)), t[:, :8]),
+                 lambda: ops.quantize_rows(torch.zeros(0, 8), ops.q8_rows(0, 8, "cpu"))):
+        with pytest.raises(ops.KernelError, match="CUDA"):
+            call()
