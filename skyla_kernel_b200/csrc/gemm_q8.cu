@@ -10,7 +10,8 @@
 //                    token's row;
 //   q8_pair_kernel   tiles of 256 tokens on two SMs, where there are many.
 // plan() chooses by what they were measured to take.
-// Every mbarrier wait is bounded: on a timeout the block records an error code (1 to 19), lets the loads it issued
+// Every mbarrier wait is bounded: on a timeout the block records an error code (1 a stage to load into, 2 a stage loaded,
+// 3 an accumulator finished, 5 one drained, 7 and 8 a cluster's exchange arrived and sent), lets the loads it issued
 // land, frees its TMEM and returns.
 #include <cuda.h>
 
@@ -443,7 +444,8 @@ q8_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // accumulators in shared memory (the ring, idle by then), and each finishes an equal part of the outputs, or of the
 // tokens, from all of them: whole numbers, so the result does not show the cut.
 // 256 tokens x 4,096 to 4,096, added, on 128 blocks of 64 columns: 9.7 us, 6.5 of them 24 KB a K block into an SM (120 GB/s,
-// what one takes in); 8,192 x 4,096 to 2 x 12,288 on 256 columns: 518 us (3,180 TOP/s; imma pipe 72 % of the active cycles).
+// what one takes in); 8,192 x 4,096 to 2 x 12,288 on 256 columns: 518 us (3,180 TOP/s).  Of 2,048 x 4,096 to 6,144 the imma
+// pipe takes 72 % of an SM's active cycles, which are 75 % of the time: whole rounds of tiles.
 constexpr int kOutBytes = BM * 128;  // 128 tokens x 128 bytes
 constexpr int kMaxSplits = 4;
 
@@ -456,7 +458,7 @@ struct TileCfg {
   static constexpr int kXBytes = BM * KB, kWBytes = BF * KB;  // of one K block
   static constexpr int kStageBytes = kKkb * (kXBytes + kWBytes);
   static constexpr int kStagesRaw = (196 * 1024) / kStageBytes;
-  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;  // 4, 3, 4
+  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;  // 4 for 256 columns, 3 for 128 (gated 6), 4 for 64
   static constexpr int kSmemBytes = kStages * kStageBytes + 2 * kOutBytes + 1024 /*align*/ + 256 /*barriers*/;
   static constexpr int kTmemCols = 2 * BF;
   static_assert(kSmemBytes + BF * 4 + 64 <= 227 * 1024, "shared memory of a block");
@@ -1171,7 +1173,8 @@ int reserve(K kernel, int bytes, Done& done) {
 
 struct RowsPlan { int rows, splits, kkb, kstack; };
 
-// How many clusters of `size` blocks run at a time (one block per SM, clusters inside a GPC).
+// How many clusters of `size` blocks run at a time (one block per SM, clusters inside a GPC).  Asked for the streaming
+// kernel; a block of the tile kernel has an SM to itself as well, so that as many of its clusters fit.
 int cluster_room(int size) {
   static Asked asked[2];
   return asked[size == 4]([size] {
@@ -1472,7 +1475,10 @@ int launch_pairs(const Operands& o, const Args& a, cudaStream_t stream) {
   return check_launch("linear_q8");
 }
 
-// The kernel of a product: tiles of p.columns (512: of two SMs; 0: weight streaming by r).
+// The kernel of a product: tiles of p.columns (512: of two SMs; 0: weight streaming by r).  Up to 16 tokens stream always.
+// (Not the best for narrow outputs of a long K that does not stack, gated or not in whole blocks: few SMs walk all of K. 16 x
+// 11,142 to 171 take 24.8 us where 17 tokens, in tiles with K over four blocks, take 8.0; 8 x 16,384 to 2 x 512 38.6, 17
+// tokens 11.3.)
 struct Plan { RowsPlan r; int bn; TilePlan p; };
 Plan plan(int M, int N, int K, bool gated, bool fours) {
   Plan c;

@@ -790,7 +790,8 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[
     itself or lies apart from it; what is written lies apart from ``weight``, ``out`` from all others.
 
     ``x`` and ``residual``: bfloat16 or float32.  A row whose sum of squares or whose products with the weight
-    leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row of zeros with ``eps = 0``."""
+    leave the 32-bit numbers, or hold a NaN, gets the scale NaN and zeros; so does a row with ``eps = 0`` whose mean
+    square is zero in 32 bits."""
     n, width, ld = _dims(x, "rmsnorm_q8") if residual is None else _written_dims(x, "rmsnorm_q8")
     code = dtype_code(x)
     if weight.dtype is not torch.float32 or weight.shape != (width,) or not weight.is_contiguous():
@@ -842,7 +843,8 @@ class Q8Weight:
     ``gated``: all gate rows, then the up rows of the same outputs.  The tensors are kept as they are if the rows
     begin on multiples of 16 bytes, else copied into such rows.  The product's kernels ask for the weight before
     they wait for the kernels ahead of them, so it is finished for good: the constructor waits for the device (and
-    refuses to run inside a stream capture), and nobody writes the tensors afterwards."""
+    refuses to run inside a stream capture), and nobody writes the tensors afterwards.  Copies, pickled and saved
+    weights come back through the constructor (``torch.load`` takes this class from its ``safe_globals``)."""
 
     __slots__ = ("rows", "gated", "n_out", "n_in", "ld", "_device", "_q", "_scale")
 
@@ -894,7 +896,8 @@ def linear_q8(x: Q8Rows, w: Q8Weight, y: torch.Tensor, mode: int = STORE,
 
     ``mode``: STORE (``y = v``, bfloat16 or float32), ACCUMULATE (``y += v``, float32), GATED (``y = silu(gate) * up``
     of a gated weight, bfloat16).  ``y`` lies apart from ``x``.  ``x``'s rows should begin on multiples of 16 bytes
-    (as :func:`q8_rows` makes them): others run on the plain kernel, with the same results."""
+    (as :func:`q8_rows` makes them): others run on the plain kernel, slowly, with the same results.  Whichever kernel
+    runs, the results are the same bits.  A gate below -87 gives zero (``silu`` is below 2^-119 there)."""
     q, scale = x
     m, k, ldx = _q8_dims(x, "linear_q8")
     if k != w.n_in:
